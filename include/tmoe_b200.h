@@ -212,6 +212,87 @@ int tmoe_ffn_gate_up(const tmoe_layer_t *layer, const void *prepared_gate, const
 int tmoe_rms_norm(int dtype, const void *x, const void *weight, float eps, int64_t T, int32_t d, void *y,
                   void *stream);
 
+/* ---- What stands around the layer in a block: its tail, its routing as data, its coefficients --------------------
+ * Forward and backward.  Pointers need the alignment of their elements only (16-byte aligned rows of a multiple of 8 elements
+ * take wider loads); last dimensions are contiguous, rows may lie any non-negative stride apart (0 repeats one row).  Outputs
+ * are dense.  Workspaces of these functions are scratch of one call: never zeroed, nothing is kept in them. */
+
+/* The tail of a block (pure_torch_mlx/model.py:25-27, 258-260, 340-341), with an optional norm behind the block:
+ *   out    = residual + layer_scale * silu(gate) * (y * rstd(y) * post_w)
+ *   normed = out * rstd(out) * next_w,                     rstd(x) = 1 / sqrt(mean(x^2) + eps)
+ * Every operand but y may be NULL: its factor or term is left out.  y, gate, layer_scale, post_w, next_w and normed have
+ * `dtype`; residual and out have `residual_dtype` (that of y, or TMOE_F32 beside bf16 blocks).  fp32 arithmetic; normed is
+ * made from the unrounded sum. */
+typedef struct tmoe_residual_norm {
+  int64_t rows;            /* 0 .. 2^30; 0 enqueues nothing */
+  int32_t d;               /* 1 .. 8192 (TMOE_ERR_UNSUPPORTED above) */
+  int32_t dtype, residual_dtype;
+  float post_eps, next_eps;
+  int32_t reserved0;
+  int64_t y_stride, residual_stride, gate_stride;  /* elements between rows */
+  const void *y, *residual, *gate;                 /* [rows, d] */
+  const void *layer_scale, *post_w, *next_w;       /* [d] */
+} tmoe_residual_norm_t;
+/* out [rows, d] (NULL: not wanted), normed [rows, d] (with next_w, and only then).  rstd: [2, rows] floats for the backward call
+ * (1/rms of y in the first row, of out in the second; each written when its weight is given), or NULL.  out may be the residual
+ * buffer itself and normed may be y's, where their rows lie d apart. */
+int tmoe_residual_norm(const tmoe_residual_norm_t *p, void *out, void *normed, float *rstd, void *stream);
+int64_t tmoe_residual_norm_workspace_bytes(const tmoe_residual_norm_t *p);   /* of the backward call */
+/* Gradients for the upstream gradients d_out (residual_dtype) and d_normed (dtype); either may be NULL (zero), not both.  Every
+ * result may be NULL (not wanted); results have the types of what they are gradients of and add nothing to what was there.
+ * `workspace` only matters for the three parameter gradients.  Bit-reproducible on one kind of GPU. */
+int tmoe_residual_norm_backward(const tmoe_residual_norm_t *p, const float *rstd, const void *d_out, int64_t d_out_stride,
+                                const void *d_normed, int64_t d_normed_stride, void *d_y, void *d_residual, void *d_gate,
+                                void *d_layer_scale, void *d_post_w, void *d_next_w, void *workspace, int64_t workspace_bytes,
+                                void *stream);
+
+/* Routing from scores [tokens, n_experts]: what tmoe_router does from the scores on, with a token mask, the tokens per expert and
+ * the two router losses.  The gate rules are tmoe_router_mode_t's, in fp32 throughout (the scores are not rounded again); equal
+ * scores go to the lower expert index.  A score of -inf switches the expert off for that token; slots without an expert get idx -1
+ * and gate 0.  A token whose mask byte is 0, or all of whose experts are off, has empty slots only and counts nowhere; its scores
+ * are not used.  With p = softmax of the logits over all experts, n = tokens that count, f_e = counts_e / (n top_k):
+ *   losses[0] = n_experts * sum_e f_e * mean_t p[t, e]     (1 when both are uniform)
+ *   losses[1] = mean_t (log sum_e exp logit[t, e])^2,   losses[2] = n   (0, 0, 0 when no token counts) */
+typedef struct tmoe_route {
+  int64_t tokens;          /* 0 .. 2^30 */
+  int32_t n_experts;       /* 1 .. 1024 (TMOE_ERR_UNSUPPORTED above) */
+  int32_t top_k;           /* 1 .. min(n_experts, TMOE_MAX_TOPK) */
+  int32_t dtype;
+  int32_t router_mode;     /* tmoe_router_mode_t */
+  float router_cap, router_temperature;
+  int64_t scores_stride;   /* elements between rows */
+  const void *scores;
+  const uint8_t *token_mask; /* [tokens], or NULL: every token counts */
+} tmoe_route_t;
+int64_t tmoe_route_workspace_bytes(const tmoe_route_t *p);   /* of the forward call */
+/* idx, gates [tokens, top_k] (descending score), counts [n_experts], losses [3] */
+int tmoe_route_tokens(const tmoe_route_t *p, int32_t *idx, float *gates, int32_t *counts, float *losses, void *workspace,
+                      int64_t workspace_bytes, void *stream);
+/* d_scores [tokens, n_experts] (dtype) from the forward call's results and the upstream gradients d_gates [tokens, top_k],
+ * d_balance and d_z (one float each, on the device); each may be NULL (zero).  counts carry no gradient. */
+int tmoe_route_tokens_backward(const tmoe_route_t *p, const int32_t *idx, const float *gates, const int32_t *counts,
+                               const float *losses, const float *d_gates, const float *d_balance, const float *d_z, void *d_scores,
+                               void *stream);
+
+/* c[t] = sum_j gates[t, j] * U_expert[idx[t, j]] (pure_torch_mlx/model.py:93 folded through the core mixing): the coefficients
+ * that tmoe_in_core takes.  A slot whose index lies outside 0 .. n_experts-1 is empty. */
+typedef struct tmoe_expert_coef {
+  int64_t tokens;          /* 0 .. 2^30 */
+  int32_t n_experts;       /* 1 .. 16384 (TMOE_ERR_UNSUPPORTED above) */
+  int32_t top_k;           /* 1 .. TMOE_MAX_TOPK */
+  int32_t r1;              /* 1 .. TMOE_MAX_R1 */
+  int32_t dtype;           /* of U_expert */
+  const int32_t *idx;      /* [tokens, top_k] */
+  const float *gates;      /* [tokens, top_k] */
+  const void *U_expert;    /* [n_experts, r1] */
+} tmoe_expert_coef_t;
+int tmoe_expert_coef(const tmoe_expert_coef_t *p, float *c, void *stream);   /* c [tokens, r1] */
+int64_t tmoe_expert_coef_workspace_bytes(const tmoe_expert_coef_t *p);        /* of the backward call */
+/* d_gates [tokens, top_k] and d_U_expert [n_experts, r1] (dtype) for d_c [tokens, r1]; either may be NULL (not wanted), not both.
+ * Bit-reproducible on one kind of GPU. */
+int tmoe_expert_coef_backward(const tmoe_expert_coef_t *p, const float *d_c, float *d_gates, void *d_U_expert, void *workspace,
+                              int64_t workspace_bytes, void *stream);
+
 /* Synchronises `stream`, reads the workspace's device status word into *device_status
  * (0, or TMOE_ERR_DEVICE_WAIT with details in the following words) and clears it. */
 int tmoe_read_device_status(void *workspace, int32_t *device_status, void *stream);

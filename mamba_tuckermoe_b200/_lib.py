@@ -23,6 +23,9 @@ EXPORTS = (
     "tmoe_prepare_factors", "tmoe_workspace_bytes", "tmoe_router", "tmoe_in_core", "tmoe_out",
     "tmoe_forward", "tmoe_read_device_status", "tmoe_launch_count", "tmoe_forward_static_scratch", "tmoe_rms_norm", "tmoe_handoff_plan",
     "tmoe_prepare_factors_prenorm", "tmoe_selftest_bounded_wait", "tmoe_ffn_gate_up",
+    "tmoe_residual_norm", "tmoe_residual_norm_workspace_bytes", "tmoe_residual_norm_backward",
+    "tmoe_route_workspace_bytes", "tmoe_route_tokens", "tmoe_route_tokens_backward",
+    "tmoe_expert_coef", "tmoe_expert_coef_workspace_bytes", "tmoe_expert_coef_backward",
     "tmoe_peer_alloc", "tmoe_peer_open", "tmoe_peer_close", "tmoe_peer_free", "tmoe_peer_push",
 )
 PEER_HANDLE_BYTES = 64
@@ -46,6 +49,25 @@ class Extras(C.Structure):
                 ("gates_out", C.c_void_p), ("c_out", C.c_void_p), ("silu_gate", C.c_void_p),
                 ("pre_norm", C.c_int32), ("pre_norm_eps", C.c_float),
                 ("n_peer_y", C.c_int32), ("reserved0", C.c_int32), ("peer_y", C.c_void_p * 7)]
+
+
+class ResidualNorm(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("d", C.c_int32), ("dtype", C.c_int32), ("residual_dtype", C.c_int32),
+                ("post_eps", C.c_float), ("next_eps", C.c_float), ("reserved0", C.c_int32),
+                ("y_stride", C.c_int64), ("residual_stride", C.c_int64), ("gate_stride", C.c_int64),
+                ("y", C.c_void_p), ("residual", C.c_void_p), ("gate", C.c_void_p),
+                ("layer_scale", C.c_void_p), ("post_w", C.c_void_p), ("next_w", C.c_void_p)]
+
+
+class Route(C.Structure):
+    _fields_ = [("tokens", C.c_int64), ("n_experts", C.c_int32), ("top_k", C.c_int32), ("dtype", C.c_int32),
+                ("router_mode", C.c_int32), ("router_cap", C.c_float), ("router_temperature", C.c_float),
+                ("scores_stride", C.c_int64), ("scores", C.c_void_p), ("token_mask", C.c_void_p)]
+
+
+class ExpertCoef(C.Structure):
+    _fields_ = [("tokens", C.c_int64), ("n_experts", C.c_int32), ("top_k", C.c_int32), ("r1", C.c_int32), ("dtype", C.c_int32),
+                ("idx", C.c_void_p), ("gates", C.c_void_p), ("U_expert", C.c_void_p)]
 
 
 class TmoeError(RuntimeError):
@@ -103,6 +125,25 @@ def load():
         lib.tmoe_forward_static_scratch.argtypes = [LP, FP, vp, i64, vp, EP, vp]
         lib.tmoe_rms_norm.restype = i32
         lib.tmoe_rms_norm.argtypes = [i32, vp, vp, C.c_float, i64, C.c_int32, vp, vp]
+        NP, RP, XP = C.POINTER(ResidualNorm), C.POINTER(Route), C.POINTER(ExpertCoef)
+        lib.tmoe_residual_norm.restype = i32
+        lib.tmoe_residual_norm.argtypes = [NP, vp, vp, vp, vp]
+        lib.tmoe_residual_norm_workspace_bytes.restype = i64
+        lib.tmoe_residual_norm_workspace_bytes.argtypes = [NP]
+        lib.tmoe_residual_norm_backward.restype = i32
+        lib.tmoe_residual_norm_backward.argtypes = [NP, vp, vp, i64, vp, i64] + [vp] * 7 + [i64, vp]
+        lib.tmoe_route_workspace_bytes.restype = i64
+        lib.tmoe_route_workspace_bytes.argtypes = [RP]
+        lib.tmoe_route_tokens.restype = i32
+        lib.tmoe_route_tokens.argtypes = [RP, vp, vp, vp, vp, vp, i64, vp]
+        lib.tmoe_route_tokens_backward.restype = i32
+        lib.tmoe_route_tokens_backward.argtypes = [RP] + [vp] * 9
+        lib.tmoe_expert_coef.restype = i32
+        lib.tmoe_expert_coef.argtypes = [XP, vp, vp]
+        lib.tmoe_expert_coef_workspace_bytes.restype = i64
+        lib.tmoe_expert_coef_workspace_bytes.argtypes = [XP]
+        lib.tmoe_expert_coef_backward.restype = i32
+        lib.tmoe_expert_coef_backward.argtypes = [XP, vp, vp, vp, vp, i64, vp]
         lib.tmoe_read_device_status.restype = i32
         lib.tmoe_read_device_status.argtypes = [vp, C.POINTER(C.c_int32), vp]
         lib.tmoe_launch_count.restype = i64
