@@ -18,6 +18,8 @@
 //   d_layer_scale = sum_t dR * v,   d_post_w = sum_t da * h,   d_next_w = sum_t dN * x
 // The two row means need one team reduction, not two: with b = dO + rstd1 * u and q = post_w * layer_scale * s * h,
 //   mean(post_w * da * h) = (sum q*b - rstd1 * mean(u*x) * sum q*x) / d.
+// The sums of d_layer_scale and d_post_w differ by a column factor only: with S = sum_t dR * s * h they are post_w * S and
+// layer_scale * S.
 // `out` is recomputed in fp32 from y, gate and residual (the same bytes as reading it back, and no rounding in between); only
 // the two rstd of a row are kept from the forward pass.
 #include "common.cuh"
@@ -29,14 +31,24 @@ namespace {
 
 constexpr int kMaxWidth = 8192;      // widest row: 512 threads x 16 elements
 constexpr int kNormThreads = 512;    // upper bound of the block size
-constexpr int kNormWarps = kNormThreads / 32;
+
+__device__ __forceinline__ void cp_async16(void *smem, const void *gmem) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ptx::smem_u32(smem)), "l"(gmem) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // VEC consecutive elements of a row as they lie in memory (VEC = 8: 16-byte loads; VEC = 1: any width, stride and base).
+// kPlanes 16-byte parts, part p of a thread at slot[p * pitch] of a shared-memory ring.
 template <typename T, int VEC> struct Piece;
 template <> struct Piece<bf16, 8> {
+  static constexpr int kPlanes = 1;
   uint4 r;
+  __device__ static __forceinline__ void copy(uint4 *slot, int, const bf16 *p) { cp_async16(slot, p); }
+  __device__ __forceinline__ void fetch(const uint4 *slot, int) { r = *slot; }
   __device__ __forceinline__ void load(const bf16 *p) { r = *reinterpret_cast<const uint4 *>(p); }
   __device__ __forceinline__ void zero() { r = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void one() { r = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u); }
   __device__ __forceinline__ float get(int q) const {
     const uint32_t w = (q >> 1) == 0 ? r.x : (q >> 1) == 1 ? r.y : (q >> 1) == 2 ? r.z : r.w;
     return __uint_as_float((q & 1) ? (w & 0xffff0000u) : (w << 16));
@@ -47,12 +59,19 @@ template <> struct Piece<bf16, 8> {
   }
 };
 template <> struct Piece<float, 8> {
+  static constexpr int kPlanes = 2;
   float4 a, b;
+  __device__ static __forceinline__ void copy(uint4 *slot, int pitch, const float *p) { cp_async16(slot, p); cp_async16(slot + pitch, p + 4); }
+  __device__ __forceinline__ void fetch(const uint4 *slot, int pitch) {
+    a = *reinterpret_cast<const float4 *>(slot);
+    b = *reinterpret_cast<const float4 *>(slot + pitch);
+  }
   __device__ __forceinline__ void load(const float *p) {
     a = reinterpret_cast<const float4 *>(p)[0];
     b = reinterpret_cast<const float4 *>(p)[1];
   }
   __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ __forceinline__ void one() { a = b = make_float4(1.f, 1.f, 1.f, 1.f); }
   __device__ __forceinline__ float get(int q) const {
     const float4 v = q < 4 ? a : b;
     return (q & 3) == 0 ? v.x : (q & 3) == 1 ? v.y : (q & 3) == 2 ? v.z : v.w;
@@ -63,9 +82,13 @@ template <> struct Piece<float, 8> {
   }
 };
 template <typename T> struct Piece<T, 1> {
+  static constexpr int kPlanes = 0;
   T r;
+  __device__ static __forceinline__ void copy(uint4 *, int, const T *) {}
+  __device__ __forceinline__ void fetch(const uint4 *, int) {}
   __device__ __forceinline__ void load(const T *p) { r = *p; }
   __device__ __forceinline__ void zero() { r = from_f32<T>(0.f); }
+  __device__ __forceinline__ void one() { r = from_f32<T>(1.f); }
   __device__ __forceinline__ float get(int) const { return to_f32(r); }
   __device__ static __forceinline__ void store(T *p, const float (&f)[1]) { *p = from_f32<T>(f[0]); }
 };
@@ -83,211 +106,330 @@ struct NormArgs {
   int64_t dos, dns;
   void *d_y, *d_res, *d_gate;                  // [rows, d]; nullptr = not wanted
   float *partial;                              // [blocks, n_sums, d] column sums; nullptr = no parameter gradient wanted
-  int sum_ls, sum_w0, sum_w1;                  // slot of each parameter gradient in `partial`, or -1
+  int sum_a, sum_x;                            // slot in `partial` of sum_t dR * s * h and of sum_t dN * x, or -1
   int n_sums;
 };
 
-// Sum over the `tw` warps of a team, in warp order; `slot` alternates between calls, so one barrier per call is enough.
-template <int N>
-__device__ __forceinline__ void team_sum(float (&v)[N], int tw, int team, float (*red)[kNormWarps][N]) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = warp_sum(v[i]);
-  if (tw == 1) return;
-  const int warp = threadIdx.x >> 5;
-  if ((threadIdx.x & 31) == 0) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) (*red)[warp][i] = v[i];
+// Sums over the `tw` warps of a team, in a fixed order.  A team has 16 places of shared memory for each sum, zero beyond its own warps
+// (TeamRed::init), which every thread reads back with wide loads; `slot` alternates between calls, so one barrier per call is enough.
+template <int N> struct TeamRed {
+  float at[2][8][N][16];   // [slot][team][sum][warp]
+  __device__ __forceinline__ void init() {
+    for (int i = threadIdx.x; i < 2 * 8 * N * 16; i += blockDim.x) (&at[0][0][0][0])[i] = 0.f;
+    __syncthreads();
   }
+};
+__device__ __forceinline__ float sum_places(const float (&v)[16], int tw) {
+  const float4 *p = reinterpret_cast<const float4 *>(v);
+  const float4 a = p[0];
+  float s = (a.x + a.y) + (a.z + a.w);
+  if (tw > 4) {
+    const float4 b = p[1];
+    s += (b.x + b.y) + (b.z + b.w);
+    if (tw > 8) {
+      const float4 c = p[2], d = p[3];
+      s += ((c.x + c.y) + (c.z + c.w)) + ((d.x + d.y) + (d.z + d.w));
+    }
+  }
+  return s;
+}
+__device__ __forceinline__ float team_sum(float v, int tw, int team, int slot, TeamRed<1> &red) {
+  v = warp_sum(v);
+  if (tw == 1) return v;
+  if ((threadIdx.x & 31) == 0) red.at[slot][team][0][(threadIdx.x >> 5) - team * tw] = v;
   ptx::named_bar_sync(1 + team, tw * 32);
-#pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = 0.f;
-  for (int w = 0; w < tw; ++w) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] += (*red)[team * tw + w][i];
-  }
+  return sum_places(red.at[slot][team][0], tw);
 }
 
-__device__ __forceinline__ float sigmoid(float g) { return 1.f / (1.f + expf(-g)); }
-
-template <typename TY, typename TR, int VEC, int NV>
-__global__ void __launch_bounds__(kNormThreads) residual_norm_kernel(const __grid_constant__ NormArgs a) {
-  __shared__ float red[2][kNormWarps][1];
-  const int tpr = a.tw * 32, team = threadIdx.x / tpr, lt = threadIdx.x - team * tpr;
-  const int64_t row = (int64_t)blockIdx.x * (blockDim.x / tpr) + team;
-  if (row >= a.rows) return;   // whole teams leave
-  const TY *y = (const TY *)a.y + row * a.ys;
-  const TY *gate = a.gate ? (const TY *)a.gate + row * a.gs : nullptr;
-  const TR *res = a.res ? (const TR *)a.res + row * a.rs : nullptr;
-  Piece<TY, VEC> py[NV], pg[NV];
-  Piece<TR, VEC> pr[NV];
+// The same for three sums at once.  The first two steps of the butterfly halve the number of values a lane carries, so three sums
+// take 6 shuffles instead of 15.
+__device__ __forceinline__ float3 team_sum3(float a, float b, float c, int tw, int team, int slot, TeamRed<3> &red) {
+  const int lane = threadIdx.x & 31;
+  const bool hi = lane & 16, up = lane & 8;
+  float p = (hi ? c : a) + __shfl_xor_sync(0xffffffffu, hi ? a : c, 16);
+  float q = (hi ? 0.f : b) + __shfl_xor_sync(0xffffffffu, hi ? b : 0.f, 16);
+  p = (up ? q : p) + __shfl_xor_sync(0xffffffffu, up ? p : q, 8);
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int e = (i * tpr + lt) * VEC;
-    py[i].zero(); pg[i].zero(); pr[i].zero();
-    if (e < a.d) {
-      py[i].load(y + e);
-      if (gate) pg[i].load(gate + e);
-      if (res) pr[i].load(res + e);
-    }
-  }
-  float rho0 = 1.f;
-  if (a.w0) {
-    float ss[1] = {0.f};
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-#pragma unroll
-      for (int q = 0; q < VEC; ++q) ss[0] = fmaf(py[i].get(q), py[i].get(q), ss[0]);
-    }
-    team_sum<1>(ss, a.tw, team, &red[0]);
-    rho0 = 1.f / sqrtf(ss[0] / (float)a.d + a.eps0);
-    if (a.rstd && lt == 0) a.rstd[row] = rho0;
-  }
-  float v[NV][VEC];
-  float ss[1] = {0.f};
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int e = (i * tpr + lt) * VEC;
-    Piece<TY, VEC> w, l;
-    w.zero(); l.zero();
-    if (e < a.d) {
-      if (a.w0) w.load((const TY *)a.w0 + e);
-      if (a.ls) l.load((const TY *)a.ls + e);
-    }
-#pragma unroll
-    for (int q = 0; q < VEC; ++q) {
-      float t = py[i].get(q);
-      if (a.w0) t = t * rho0 * w.get(q);
-      if (gate) { const float g = pg[i].get(q); t *= g * sigmoid(g); }
-      if (a.ls) t *= l.get(q);
-      t += pr[i].get(q);
-      v[i][q] = t;
-      ss[0] = fmaf(t, t, ss[0]);
-    }
-    if (a.out && e < a.d) Piece<TR, VEC>::store((TR *)a.out + row * a.d + e, v[i]);
-  }
-  if (!a.normed) return;
-  team_sum<1>(ss, a.tw, team, &red[1]);
-  const float rho1 = 1.f / sqrtf(ss[0] / (float)a.d + a.eps1);
-  if (a.rstd && lt == 0) a.rstd[a.rows + row] = rho1;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int e = (i * tpr + lt) * VEC;
-    if (e < a.d) {
-      Piece<TY, VEC> w;
-      w.load((const TY *)a.w1 + e);
-#pragma unroll
-      for (int q = 0; q < VEC; ++q) v[i][q] = v[i][q] * rho1 * w.get(q);
-      Piece<TY, VEC>::store((TY *)a.normed + row * a.d + e, v[i]);
-    }
-  }
+  for (int o = 4; o > 0; o >>= 1) p += __shfl_xor_sync(0xffffffffu, p, o);
+  // lanes 0.. hold a, 8.. b, 16.. c
+  if (tw == 1)
+    return make_float3(__shfl_sync(0xffffffffu, p, 0), __shfl_sync(0xffffffffu, p, 8), __shfl_sync(0xffffffffu, p, 16));
+  if ((lane & 7) == 0 && lane < 24) red.at[slot][team][lane >> 3][(threadIdx.x >> 5) - team * tw] = p;
+  ptx::named_bar_sync(1 + team, tw * 32);
+  return make_float3(sum_places(red.at[slot][team][0], tw), sum_places(red.at[slot][team][1], tw), sum_places(red.at[slot][team][2], tw));
 }
 
-// A team walks over rows blockIdx * teams + team, + gridDim * teams, ...; every thread owns the same columns in all of them, so
-// the parameter gradients are sums in its registers.  At the end a block adds its teams in order and writes one row of partial
-// sums; norm_params_kernel adds the blocks in order.  The result depends on the sizes and the grid only.
-template <typename TY, typename TR, int VEC, int NV>
-__global__ void __launch_bounds__(kNormThreads) residual_norm_backward_kernel(const __grid_constant__ NormArgs a) {
-  __shared__ float red[2][kNormWarps][3];
-  extern __shared__ float fold[];   // [d] when a block has several teams
-  const int tpr = a.tw * 32, team = threadIdx.x / tpr, lt = threadIdx.x - team * tpr, teams = blockDim.x / tpr;
-  float acc_ls[NV][VEC], acc_w0[NV][VEC], acc_w1[NV][VEC];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-#pragma unroll
-    for (int q = 0; q < VEC; ++q) acc_ls[i][q] = acc_w0[i][q] = acc_w1[i][q] = 0.f;
-  }
-  const float inv_d = 1.f / (float)a.d;
-  int slot = 0;
-  for (int64_t row = (int64_t)blockIdx.x * teams + team; row < a.rows; row += (int64_t)gridDim.x * teams) {
-    const TY *y = (const TY *)a.y + row * a.ys;
-    const TY *gate = a.gate ? (const TY *)a.gate + row * a.gs : nullptr;
-    const TR *res = a.res ? (const TR *)a.res + row * a.rs : nullptr;
-    const TR *d_out = a.d_out ? (const TR *)a.d_out + row * a.dos : nullptr;
-    const TY *d_n = a.d_normed ? (const TY *)a.d_normed + row * a.dns : nullptr;
-    Piece<TY, VEC> py[NV], pg[NV], pn[NV];
-    Piece<TR, VEC> pr[NV], po[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int e = (i * tpr + lt) * VEC;
-      py[i].zero(); pg[i].zero(); pr[i].zero(); po[i].zero(); pn[i].zero();
-      if (e < a.d) {
-        py[i].load(y + e);
-        if (gate) pg[i].load(gate + e);
-        if (res) pr[i].load(res + e);
-        if (d_out) po[i].load(d_out + e);
-        if (d_n) pn[i].load(d_n + e);
-      }
-    }
-    const float rho0 = a.w0 ? a.rstd[row] : 1.f;
-    const float rho1 = d_n ? a.rstd[a.rows + row] : 0.f;   // without dN nothing flows through the next norm
-    float s3[3] = {0.f, 0.f, 0.f};                          // sum u*x, sum q*b, sum q*x
-    if (d_n || a.w0) {
+// exp and reciprocal to a few ulp: the gate is one factor of a sum that is rounded to the storage type
+__device__ __forceinline__ float sigmoid(float g) { return __fdividef(1.f, 1.f + __expf(-g)); }
+
+// One row's inputs as they lie in memory.  Where the ring has stages, a row's pieces are copied to shared memory some rows ahead; a
+// thread copies and reads its own pieces only, so the ring needs no barrier, just the thread's own wait for its copies.
+template <typename TY, typename TR, int VEC, int NV, bool GATE, bool BACK> struct RowIn {
+  using PY = Piece<TY, VEC>;
+  using PR = Piece<TR, VEC>;
+  static constexpr int kPlanes = NV * ((1 + (GATE ? 1 : 0) + (BACK ? 1 : 0)) * PY::kPlanes + (BACK ? 2 : 1) * PR::kPlanes);
+  // as many rows ahead as 192 KB hold for the warps that an SM is meant to run; below 2 stages rows are loaded when their turn comes
+  static constexpr int kWarps = BACK || NV == 2 ? 16 : 32;
+  static constexpr int kFit = kPlanes ? 196608 / (kPlanes * kWarps * 512) : 0;
+  static constexpr int kStages = kFit >= 3 ? 3 : kFit == 2 ? 2 : 1;
+  static constexpr bool kRing = kStages > 1;
+  PY y[NV], g[GATE ? NV : 1], dn[BACK ? NV : 1];
+  PR r[NV], dout[BACK ? NV : 1];
+
+  __device__ static __forceinline__ void copy(const NormArgs &a, int64_t row, int tpr, int lt, uint4 *slot, int pitch) {
+    if (row < a.rows) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int e = (i * tpr + lt) * VEC;
-        Piece<TY, VEC> w0, l, w1;
-        w0.zero(); l.zero(); w1.zero();
         if (e < a.d) {
-          if (a.w0) w0.load((const TY *)a.w0 + e);
-          if (a.ls) l.load((const TY *)a.ls + e);
-          if (d_n) w1.load((const TY *)a.w1 + e);
-        }
-#pragma unroll
-        for (int q = 0; q < VEC; ++q) {
-          const float h = py[i].get(q) * rho0;
-          float c = a.ls ? l.get(q) : 1.f;                  // d out / d a
-          if (gate) { const float g = pg[i].get(q); c *= g * sigmoid(g); }
-          const float w = a.w0 ? w0.get(q) : 1.f;
-          const float x = fmaf(c * w, h, pr[i].get(q)) * rho1;
-          const float u = w1.get(q) * pn[i].get(q);
-          const float b = fmaf(rho1, u, po[i].get(q)), qq = c * w * h;
-          s3[0] = fmaf(u, x, s3[0]);
-          s3[1] = fmaf(qq, b, s3[1]);
-          s3[2] = fmaf(qq, x, s3[2]);
+          PY::copy(slot, pitch, (const TY *)a.y + row * a.ys + e);
+          slot += PY::kPlanes * pitch;
+          if (GATE) { PY::copy(slot, pitch, (const TY *)a.gate + row * a.gs + e); slot += PY::kPlanes * pitch; }
+          if (BACK) { if (a.d_normed) PY::copy(slot, pitch, (const TY *)a.d_normed + row * a.dns + e); slot += PY::kPlanes * pitch; }
+          if (a.res) PR::copy(slot, pitch, (const TR *)a.res + row * a.rs + e);
+          slot += PR::kPlanes * pitch;
+          if (BACK) { if (a.d_out) PR::copy(slot, pitch, (const TR *)a.d_out + row * a.dos + e); slot += PR::kPlanes * pitch; }
         }
       }
-      team_sum<3>(s3, a.tw, team, &red[slot]);
-      slot ^= 1;
     }
-    const float m1 = s3[0] * inv_d;
-    const float m0 = (s3[1] - rho1 * m1 * s3[2]) * inv_d;
+    cp_async_commit();
+  }
+  __device__ __forceinline__ void fetch(const NormArgs &a, int tpr, int lt, const uint4 *slot, int pitch) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int e = (i * tpr + lt) * VEC;
-      if (e < a.d) {
-        Piece<TY, VEC> w0, l, w1;
-        w0.zero(); l.zero(); w1.zero();
-        if (a.w0) w0.load((const TY *)a.w0 + e);
-        if (a.ls) l.load((const TY *)a.ls + e);
-        if (d_n) w1.load((const TY *)a.w1 + e);
-        float f_y[VEC], f_r[VEC], f_g[VEC];
-#pragma unroll
-        for (int q = 0; q < VEC; ++q) {
-          const float h = py[i].get(q) * rho0, w = a.w0 ? w0.get(q) : 1.f, ls = a.ls ? l.get(q) : 1.f;
-          const float g = pg[i].get(q), sg = gate ? sigmoid(g) : 0.f, s = gate ? g * sg : 1.f;
-          const float aa = h * w, v = aa * s;
-          const float x = fmaf(ls, v, pr[i].get(q)) * rho1;
-          const float dn = pn[i].get(q), u = w1.get(q) * dn;
-          const float dr = po[i].get(q) + rho1 * (u - x * m1);
-          const float dv = ls * dr, da = dv * s;
-          f_r[q] = dr;
-          f_g[q] = dv * aa * (sg * (1.f + g * (1.f - sg)));
-          f_y[q] = a.w0 ? rho0 * (w * da - h * m0) : da;
-          acc_ls[i][q] = fmaf(dr, v, acc_ls[i][q]);
-          acc_w0[i][q] = fmaf(da, h, acc_w0[i][q]);
-          acc_w1[i][q] = fmaf(dn, x, acc_w1[i][q]);
-        }
-        if (a.d_y) Piece<TY, VEC>::store((TY *)a.d_y + row * a.d + e, f_y);
-        if (a.d_res) Piece<TR, VEC>::store((TR *)a.d_res + row * a.d + e, f_r);
-        if (a.d_gate) Piece<TY, VEC>::store((TY *)a.d_gate + row * a.d + e, f_g);
+      y[i].zero(); r[i].zero();
+      if (GATE) g[i].zero();
+      if (BACK) { dn[i].zero(); dout[i].zero(); }
+      if ((i * tpr + lt) * VEC < a.d) {
+        y[i].fetch(slot, pitch);
+        slot += PY::kPlanes * pitch;
+        if (GATE) { g[i].fetch(slot, pitch); slot += PY::kPlanes * pitch; }
+        if (BACK) { if (a.d_normed) dn[i].fetch(slot, pitch); slot += PY::kPlanes * pitch; }
+        if (a.res) r[i].fetch(slot, pitch);
+        slot += PR::kPlanes * pitch;
+        if (BACK) { if (a.d_out) dout[i].fetch(slot, pitch); slot += PR::kPlanes * pitch; }
       }
     }
   }
+  __device__ __forceinline__ void load(const NormArgs &a, int64_t row, int tpr, int lt) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int e = (i * tpr + lt) * VEC;
+      y[i].zero(); r[i].zero();
+      if (GATE) g[i].zero();
+      if (BACK) { dn[i].zero(); dout[i].zero(); }
+      if (e < a.d) {
+        y[i].load((const TY *)a.y + row * a.ys + e);
+        if (a.res) r[i].load((const TR *)a.res + row * a.rs + e);
+        if (GATE) g[i].load((const TY *)a.gate + row * a.gs + e);
+        if (BACK) {
+          if (a.d_out) dout[i].load((const TR *)a.d_out + row * a.dos + e);
+          if (a.d_normed) dn[i].load((const TY *)a.d_normed + row * a.dns + e);
+        }
+      }
+    }
+  }
+};
+
+// The rows of one team, one after the other.
+template <typename In> struct RowWalk {
+  uint4 *slot;
+  int64_t step;
+  int stage;
+  __device__ __forceinline__ RowWalk(const NormArgs &a, int64_t row, int64_t step_, uint4 *ring, int tpr, int lt)
+      : slot(ring + threadIdx.x), step(step_), stage(0) {
+    if (In::kRing) {
+#pragma unroll
+      for (int s = 0; s < In::kStages - 1; ++s) In::copy(a, row + s * step, tpr, lt, at(s), blockDim.x);
+    }
+  }
+  __device__ __forceinline__ uint4 *at(int s) const { return slot + s * In::kPlanes * blockDim.x; }
+  __device__ __forceinline__ void take(const NormArgs &a, int64_t row, int tpr, int lt, In &in) {
+    if (In::kRing) {
+      const int last = stage == 0 ? In::kStages - 1 : stage - 1;
+      In::copy(a, row + (In::kStages - 1) * step, tpr, lt, at(last), blockDim.x);
+      cp_async_wait<In::kStages - 1>();
+      in.fetch(a, tpr, lt, at(stage), blockDim.x);
+      stage = stage + 1 == In::kStages ? 0 : stage + 1;
+    } else {
+      in.load(a, row, tpr, lt);
+    }
+  }
+};
+
+// The parameter vectors' columns of one thread (1 where a factor is absent).  With 8 columns a thread they stay in registers over all
+// its rows; with 16 they are read again (from L1) for each, which is cheaper than the spills they cause.
+template <typename TY, int VEC, int NV> struct Params {
+  Piece<TY, VEC> w0[NV], ls[NV], w1[NV];
+  __device__ __forceinline__ void load(const NormArgs &a, int tpr, int lt) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int e = (i * tpr + lt) * VEC;
+      w0[i].zero(); ls[i].zero(); w1[i].zero();
+      if (e < a.d) {
+        if (a.w0) w0[i].load((const TY *)a.w0 + e); else w0[i].one();
+        if (a.ls) ls[i].load((const TY *)a.ls + e); else ls[i].one();
+        if (a.w1) w1[i].load((const TY *)a.w1 + e);
+      }
+    }
+  }
+};
+
+extern __shared__ uint4 norm_ring[];
+
+// A team walks over rows blockIdx * teams + team, + gridDim * teams, ...
+template <typename TY, typename TR, int VEC, int NV, bool GATE>
+__global__ void __launch_bounds__(kNormThreads, NV == 1 && VEC == 8 ? 2 : 1) residual_norm_kernel(const __grid_constant__ NormArgs a) {
+  using In = RowIn<TY, TR, VEC, NV, GATE, false>;
+  __shared__ __align__(16) TeamRed<1> red;
+  red.init();
+  const int tpr = a.tw * 32, team = threadIdx.x / tpr, lt = threadIdx.x - team * tpr;
+  const int64_t step = (int64_t)gridDim.x * (blockDim.x / tpr);
+  int64_t row = (int64_t)blockIdx.x * (blockDim.x / tpr) + team;
+  const float inv_d = 1.f / (float)a.d;
+  RowWalk<In> walk(a, row, step, norm_ring, tpr, lt);
+  Params<TY, VEC, NV> w;
+  w.load(a, tpr, lt);
+  int slot = 0;
+  for (; row < a.rows; row += step) {
+    In in;
+    walk.take(a, row, tpr, lt, in);
+    float rho0 = 1.f;
+    if (a.w0) {
+      float ss = 0.f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) ss = fmaf(in.y[i].get(q), in.y[i].get(q), ss);
+      }
+      ss = team_sum(ss, a.tw, team, slot, red);
+      slot ^= 1;
+      rho0 = rsqrtf(fmaf(ss, inv_d, a.eps0));
+      if (a.rstd && lt == 0) a.rstd[row] = rho0;
+    }
+    float v[NV][VEC], ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+#pragma unroll
+      for (int q = 0; q < VEC; ++q) {
+        float t = in.y[i].get(q) * rho0 * w.w0[i].get(q);
+        if (GATE) { const float g = in.g[i].get(q); t *= g * sigmoid(g); }
+        t = fmaf(t, w.ls[i].get(q), in.r[i].get(q));
+        v[i][q] = t;
+        ss = fmaf(t, t, ss);
+      }
+      const int e = (i * tpr + lt) * VEC;
+      if (a.out && e < a.d) Piece<TR, VEC>::store((TR *)a.out + row * a.d + e, v[i]);
+    }
+    if (!a.normed) continue;
+    ss = team_sum(ss, a.tw, team, slot, red);
+    slot ^= 1;
+    const float rho1 = rsqrtf(fmaf(ss, inv_d, a.eps1));
+    if (a.rstd && lt == 0) a.rstd[a.rows + row] = rho1;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int e = (i * tpr + lt) * VEC;
+#pragma unroll
+      for (int q = 0; q < VEC; ++q) v[i][q] *= rho1 * w.w1[i].get(q);
+      if (e < a.d) Piece<TY, VEC>::store((TY *)a.normed + row * a.d + e, v[i]);
+    }
+  }
+}
+
+// The same walk; every thread owns the same columns in all rows, so the parameter gradients are sums in its registers:
+// d_next_w = sum dN * x, and d_layer_scale and d_post_w are post_w and layer_scale times the same sum dR * s * h.  At the end a block
+// adds its teams in order and writes one row of partial sums; norm_params_kernel adds the blocks in order.  The result depends on the
+// sizes and the grid only.
+template <typename TY, typename TR, int VEC, int NV, bool GATE>
+__global__ void __launch_bounds__(kNormThreads) residual_norm_backward_kernel(const __grid_constant__ NormArgs a) {
+  using In = RowIn<TY, TR, VEC, NV, GATE, true>;
+  __shared__ __align__(16) TeamRed<3> red;
+  red.init();
+  const int tpr = a.tw * 32, team = threadIdx.x / tpr, lt = threadIdx.x - team * tpr, teams = blockDim.x / tpr;
+  const int64_t step = (int64_t)gridDim.x * teams;
+  int64_t row = (int64_t)blockIdx.x * teams + team;
+  const float inv_d = 1.f / (float)a.d;
+  RowWalk<In> walk(a, row, step, norm_ring, tpr, lt);
+  constexpr bool kKeep = NV * VEC <= 8;
+  Params<TY, VEC, NV> w;
+  w.load(a, tpr, lt);
+  float acc_a[NV][VEC], acc_x[NV][VEC];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+#pragma unroll
+    for (int q = 0; q < VEC; ++q) acc_a[i][q] = acc_x[i][q] = 0.f;
+  }
+  int slot = 0;
+  // without dN nothing flows through the next norm; one row's rstd are loaded a row ahead
+  float next0 = a.w0 && row < a.rows ? a.rstd[row] : 1.f, next1 = a.d_normed && row < a.rows ? a.rstd[a.rows + row] : 0.f;
+  for (; row < a.rows; row += step) {
+    const float rho0 = next0, rho1 = next1;
+    if (row + step < a.rows) {
+      if (a.w0) next0 = a.rstd[row + step];
+      if (a.d_normed) next1 = a.rstd[a.rows + row + step];
+    }
+    In in;
+    walk.take(a, row, tpr, lt, in);
+    if (!kKeep) w.load(a, tpr, lt);
+    float x[NV][VEC], b[NV][VEC], s1 = 0.f, s2 = 0.f, s3 = 0.f;   // sum u*x, sum q*b, sum q*x
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+#pragma unroll
+      for (int q = 0; q < VEC; ++q) {
+        float t = in.y[i].get(q) * rho0 * w.w0[i].get(q) * w.ls[i].get(q);
+        if (GATE) { const float g = in.g[i].get(q); t *= g * sigmoid(g); }
+        x[i][q] = (in.r[i].get(q) + t) * rho1;
+        const float u = w.w1[i].get(q) * in.dn[i].get(q);
+        b[i][q] = fmaf(rho1, u, in.dout[i].get(q));
+        s1 = fmaf(u, x[i][q], s1);
+        s2 = fmaf(t, b[i][q], s2);
+        s3 = fmaf(t, x[i][q], s3);
+      }
+    }
+    float k1 = 0.f, k0 = 0.f;
+    if (a.w0 || a.d_normed) {
+      const float3 r = team_sum3(s1, s2, s3, a.tw, team, slot, red);
+      slot ^= 1;
+      k1 = rho1 * r.x * inv_d;
+      k0 = a.w0 ? rho0 * inv_d * (r.y - k1 * r.z) : 0.f;
+    }
+    if (!kKeep) w.load(a, tpr, lt);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int e = (i * tpr + lt) * VEC;
+      float f[VEC];
+#pragma unroll
+      for (int q = 0; q < VEC; ++q) {
+        b[i][q] = fmaf(-k1, x[i][q], b[i][q]);                        // dR
+        acc_x[i][q] = fmaf(in.dn[i].get(q), x[i][q], acc_x[i][q]);
+      }
+      if (a.d_res && e < a.d) Piece<TR, VEC>::store((TR *)a.d_res + row * a.d + e, b[i]);
+      if (GATE) {
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) {
+          const float g = in.g[i].get(q), sg = sigmoid(g), h = in.y[i].get(q) * rho0;
+          f[q] = b[i][q] * w.ls[i].get(q) * w.w0[i].get(q) * h * (sg * fmaf(g, 1.f - sg, 1.f));
+          b[i][q] *= g * sg;                                           // dR * s
+        }
+        if (a.d_gate && e < a.d) Piece<TY, VEC>::store((TY *)a.d_gate + row * a.d + e, f);
+      }
+#pragma unroll
+      for (int q = 0; q < VEC; ++q) {
+        const float h = in.y[i].get(q) * rho0;
+        acc_a[i][q] = fmaf(b[i][q], h, acc_a[i][q]);
+        f[q] = fmaf(b[i][q] * rho0, w.w0[i].get(q) * w.ls[i].get(q), -k0 * h);
+      }
+      if (a.d_y && e < a.d) Piece<TY, VEC>::store((TY *)a.d_y + row * a.d + e, f);
+    }
+  }
   if (!a.partial) return;
+  // [d] floats where the ring was, when a block has several teams: all of its copies have landed and been read by then
+  cp_async_wait<0>();
+  float *fold = reinterpret_cast<float *>(norm_ring);
   float *dst = a.partial + (int64_t)blockIdx.x * a.n_sums * a.d;
 #pragma unroll
-  for (int k = 0; k < 3; ++k) {
-    const int at = k == 0 ? a.sum_ls : k == 1 ? a.sum_w0 : a.sum_w1;
+  for (int k = 0; k < 2; ++k) {
+    const int at = k == 0 ? a.sum_a : a.sum_x;
     if (at < 0) continue;
     for (int m = 0; m < teams; ++m) {            // teams add themselves to the block's row one after the other
       if (teams > 1) __syncthreads();
@@ -298,7 +440,7 @@ __global__ void __launch_bounds__(kNormThreads) residual_norm_backward_kernel(co
           if (e < a.d) {
 #pragma unroll
             for (int q = 0; q < VEC; ++q) {
-              float t = k == 0 ? acc_ls[i][q] : k == 1 ? acc_w0[i][q] : acc_w1[i][q];
+              float t = k == 0 ? acc_a[i][q] : acc_x[i][q];
               if (m > 0) t += fold[e + q];
               if (m == teams - 1) dst[(int64_t)at * a.d + e + q] = t;
               else fold[e + q] = t;
@@ -311,43 +453,40 @@ __global__ void __launch_bounds__(kNormThreads) residual_norm_backward_kernel(co
 }
 
 // Sum of the blocks' partial rows, one column per thread column of a 32 x 8 block: each of the 8 rows of threads adds every
-// eighth block's value, then the eight are added in order.
+// eighth block's value, then the eight are added in order and turned into the parameter gradients.
 template <typename TY>
-__global__ void __launch_bounds__(256) norm_params_kernel(const float *__restrict__ partial, int blocks, int n_sums, int d,
-                                                          TY *d_ls, TY *d_w0, TY *d_w1, int s_ls, int s_w0, int s_w1) {
+__global__ void __launch_bounds__(256) norm_params_kernel(const __grid_constant__ NormArgs a, int blocks, TY *d_ls, TY *d_w0, TY *d_w1) {
   __shared__ float part[8][33];
-  const int col = blockIdx.x * 32 + (threadIdx.x & 31), lane = threadIdx.x & 31, part_i = threadIdx.x >> 5;
-  const int n = n_sums * d;
+  const int lane = threadIdx.x & 31, col = blockIdx.x * 32 + lane, part_i = threadIdx.x >> 5;
+  const int n = a.n_sums * a.d;
   float s = 0.f;
   if (col < n)
-    for (int b = part_i; b < blocks; b += 8) s += partial[(int64_t)b * n + col];
+    for (int b = part_i; b < blocks; b += 8) s += a.partial[(int64_t)b * n + col];
   part[part_i][lane] = s;
   __syncthreads();
   if (part_i == 0 && col < n) {
     float t = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) t += part[i][lane];
-    const int which = col / d, e = col - which * d;
-    TY *dst = which == s_ls ? d_ls : which == s_w0 ? d_w0 : d_w1;
-    dst[e] = from_f32<TY>(t);
+    const int which = col / a.d, e = col - which * a.d;
+    if (which == a.sum_x) {
+      d_w1[e] = from_f32<TY>(t);
+    } else {
+      if (d_ls) d_ls[e] = from_f32<TY>(a.w0 ? t * to_f32(((const TY *)a.w0)[e]) : t);
+      if (d_w0) d_w0[e] = from_f32<TY>(a.ls ? t * to_f32(((const TY *)a.ls)[e]) : t);
+    }
   }
 }
 
 struct NormShape { int tw, nv, teams; };
 
-// Warps per row and 8-element pieces per thread.  Up to 1024 columns one warp owns a row (no barriers); wider rows are shared by
-// just enough warps for two pieces per thread.
-NormShape norm_shape(int d, int max_nv1) {
+// Warps per row, pieces per thread, rows worked on at once by a block.  One 8-element piece per thread up to 4096 columns: a row
+// spread over several warps costs a barrier, but leaves registers for the next row's loads and enough warps on an SM.
+NormShape norm_shape(int d) {
   NormShape s;
   const int pieces = (d + 7) / 8;
-  if (pieces <= 32 * max_nv1) {
-    s.tw = 1;
-    s.nv = (pieces + 31) / 32;
-    if (s.nv == 3) s.nv = 4;
-  } else {
-    s.nv = pieces <= 256 ? 1 : 2;
-    s.tw = (pieces + 32 * s.nv - 1) / (32 * s.nv);
-  }
+  s.nv = pieces <= 512 ? 1 : 2;
+  s.tw = (pieces + 32 * s.nv - 1) / (32 * s.nv);
   s.teams = s.tw >= 8 ? 1 : 8 / s.tw;
   return s;
 }
@@ -379,7 +518,7 @@ NormArgs norm_args(const tmoe_residual_norm_t &p) {
   a.y = p.y; a.res = p.residual; a.ls = p.layer_scale; a.gate = p.gate; a.w0 = p.post_w; a.w1 = p.next_w;
   a.ys = p.y_stride; a.rs = p.residual_stride; a.gs = p.gate_stride;
   a.rows = p.rows; a.d = p.d; a.eps0 = p.post_eps; a.eps1 = p.next_eps;
-  a.sum_ls = a.sum_w0 = a.sum_w1 = -1;
+  a.sum_a = a.sum_x = -1;
   return a;
 }
 
@@ -391,37 +530,64 @@ bool norm_wide(const tmoe_residual_norm_t &p) {
          wide_ok(p.next_w, 0, sy);
 }
 
-template <typename TY, typename TR>
-void launch_forward(const NormArgs &a0, bool wide, cudaStream_t st) {
-  NormArgs a = a0;
-  const NormShape s = norm_shape(a.d, 4);
-  a.tw = s.tw;
-  const dim3 grid((unsigned)((a.rows + s.teams - 1) / s.teams)), block(s.teams * s.tw * 32);
-#define TMOE_RN(V, N) residual_norm_kernel<TY, TR, V, N><<<grid, block, 0, st>>>(a)
-  if (wide) { if (s.nv == 1) TMOE_RN(8, 1); else if (s.nv == 2) TMOE_RN(8, 2); else TMOE_RN(8, 4); }
-  else { if (s.nv == 1) TMOE_RN(1, 8); else if (s.nv == 2) TMOE_RN(1, 16); else TMOE_RN(1, 32); }
-#undef TMOE_RN
-}
-
-NormShape backward_shape(int d) { return norm_shape(d, 1); }
-int backward_blocks(int64_t rows, int d, int sms) {
-  const NormShape s = backward_shape(d);
-  const int64_t want = (rows + s.teams - 1) / s.teams, cap = (int64_t)sms * (s.tw * s.teams > 8 ? 1 : 2);
+// Blocks of the walk: as many as are resident at once (32 warps an SM forward, 16 backward), no more than there are rows for
+int norm_blocks(int64_t rows, int d, bool back, int sms) {
+  const NormShape s = norm_shape(d);
+  const int warps = s.tw * s.teams, resident = back || s.nv == 2 ? 16 : 32;
+  const int64_t want = (rows + s.teams - 1) / s.teams, cap = (int64_t)sms * (resident / warps);
   return (int)(want < cap ? want : cap);
 }
 
-template <typename TY, typename TR>
-void launch_backward(const NormArgs &a0, bool wide, int blocks, cudaStream_t st) {
-  NormArgs a = a0;
-  const NormShape s = backward_shape(a.d);
-  a.tw = s.tw;
-  const dim3 grid((unsigned)blocks), block(s.teams * s.tw * 32);
-  const size_t smem = s.teams > 1 ? (size_t)a.d * 4 : 0;
-#define TMOE_RNB(V, N) residual_norm_backward_kernel<TY, TR, V, N><<<grid, block, smem, st>>>(a)
+// Launch with `smem` bytes of dynamic shared memory; the opt-in above 48 KB (static part included) is made once per
+// kernel and device
+template <typename In, typename Kernel>
+void launch_walk(Kernel kernel, const NormArgs &a, const NormShape &s, int blocks, bool fold, cudaStream_t st) {
+  static std::atomic<uint64_t> opted{0};
+  const int threads = s.teams * s.tw * 32;
+  size_t smem = In::kRing ? (size_t)In::kStages * In::kPlanes * threads * 16 : 0;
+  if (fold && s.teams > 1 && smem < (size_t)a.d * 4) smem = (size_t)a.d * 4;
+  if (smem > 46 * 1024) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (!(opted.load(std::memory_order_relaxed) & bit)) {
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+      opted.fetch_or(bit, std::memory_order_relaxed);
+    }
+  }
+  kernel<<<blocks, threads, smem, st>>>(a);
+}
+
+template <typename TY, typename TR, bool GATE>
+void launch_forward(const NormArgs &a, const NormShape &s, bool wide, int blocks, cudaStream_t st) {
+#define TMOE_RN(V, N) launch_walk<RowIn<TY, TR, V, N, GATE, false>>(residual_norm_kernel<TY, TR, V, N, GATE>, a, s, blocks, false, st)
+  if (wide) { if (s.nv == 1) TMOE_RN(8, 1); else TMOE_RN(8, 2); }
+  else { if (s.nv == 1) TMOE_RN(1, 8); else TMOE_RN(1, 16); }
+#undef TMOE_RN
+}
+
+template <typename TY, typename TR, bool GATE>
+void launch_backward(const NormArgs &a, const NormShape &s, bool wide, int blocks, cudaStream_t st) {
+#define TMOE_RNB(V, N) launch_walk<RowIn<TY, TR, V, N, GATE, true>>(residual_norm_backward_kernel<TY, TR, V, N, GATE>, a, s, blocks, true, st)
   if (wide) { if (s.nv == 1) TMOE_RNB(8, 1); else TMOE_RNB(8, 2); }
   else { if (s.nv == 1) TMOE_RNB(1, 8); else TMOE_RNB(1, 16); }
 #undef TMOE_RNB
 }
+
+// CALL<y type, residual type, gate>(...) for the call's types
+#define TMOE_NORM_TYPES(CALL, p, ...)                                              \
+  do {                                                                             \
+    if ((p)->dtype == TMOE_F32) {                                                  \
+      if ((p)->gate) CALL<float, float, true>(__VA_ARGS__);                        \
+      else CALL<float, float, false>(__VA_ARGS__);                                 \
+    } else if ((p)->residual_dtype == TMOE_F32) {                                  \
+      if ((p)->gate) CALL<bf16, float, true>(__VA_ARGS__);                         \
+      else CALL<bf16, float, false>(__VA_ARGS__);                                  \
+    } else {                                                                       \
+      if ((p)->gate) CALL<bf16, bf16, true>(__VA_ARGS__);                          \
+      else CALL<bf16, bf16, false>(__VA_ARGS__);                                   \
+    }                                                                              \
+  } while (0)
 
 }  // namespace
 }  // namespace tmoe
@@ -442,9 +608,11 @@ int tmoe_residual_norm(const tmoe_residual_norm_t *p, void *out, void *normed, f
   a.out = out; a.normed = normed; a.rstd = rstd;
   const bool wide = norm_wide(*p) && wide_ok(out, p->d, sr) && wide_ok(normed, p->d, sy);
   cudaStream_t st = (cudaStream_t)stream;
-  if (p->dtype == TMOE_F32) launch_forward<float, float>(a, wide, st);
-  else if (p->residual_dtype == TMOE_F32) launch_forward<bf16, float>(a, wide, st);
-  else launch_forward<bf16, bf16>(a, wide, st);
+  const int sms = current_device_sms();
+  if (sms <= 0) return TMOE_ERR_CUDA;
+  const NormShape s = norm_shape(p->d);
+  a.tw = s.tw;
+  TMOE_NORM_TYPES(launch_forward, p, a, s, wide, norm_blocks(p->rows, p->d, false, sms), st);
   count_launch();
   return launch_status();
 }
@@ -453,7 +621,7 @@ int64_t tmoe_residual_norm_workspace_bytes(const tmoe_residual_norm_t *p) {
   int rc = check_norm(p);
   if (rc) return rc;
   // sized for up to 160 SMs, whatever device the sizing query runs on
-  return p->rows == 0 ? 0 : (int64_t)backward_blocks(p->rows, p->d, 160) * 3 * p->d * 4;
+  return p->rows == 0 ? 0 : (int64_t)norm_blocks(p->rows, p->d, true, 160) * 2 * p->d * 4;
 }
 
 int tmoe_residual_norm_backward(const tmoe_residual_norm_t *p, const float *rstd, const void *d_out, int64_t d_out_stride,
@@ -486,12 +654,11 @@ int tmoe_residual_norm_backward(const tmoe_residual_norm_t *p, const float *rstd
   a.rstd = const_cast<float *>(rstd);
   a.d_out = d_out; a.dos = d_out_stride; a.d_normed = d_normed; a.dns = d_normed_stride;
   a.d_y = d_y; a.d_res = d_residual; a.d_gate = d_gate;
-  if (d_layer_scale) a.sum_ls = a.n_sums++;
-  if (d_post_w) a.sum_w0 = a.n_sums++;
-  if (d_next_w) a.sum_w1 = a.n_sums++;
+  if (d_layer_scale || d_post_w) a.sum_a = a.n_sums++;
+  if (d_next_w) a.sum_x = a.n_sums++;
   const int sms = current_device_sms();
   if (sms <= 0) return TMOE_ERR_CUDA;
-  const int blocks = backward_blocks(p->rows, p->d, sms < 160 ? sms : 160);
+  const int blocks = norm_blocks(p->rows, p->d, true, sms < 160 ? sms : 160);
   if (params) {
     if (!workspace) return TMOE_ERR_NULL;
     if (workspace_bytes < (int64_t)blocks * a.n_sums * p->d * 4) return TMOE_ERR_WORKSPACE;
@@ -499,19 +666,17 @@ int tmoe_residual_norm_backward(const tmoe_residual_norm_t *p, const float *rstd
   }
   const bool wide = norm_wide(*p) && wide_ok(d_out, d_out_stride, sr) && wide_ok(d_normed, d_normed_stride, sy) &&
                     wide_ok(d_y, p->d, sy) && wide_ok(d_residual, p->d, sr) && wide_ok(d_gate, p->d, sy);
-  if (p->dtype == TMOE_F32) launch_backward<float, float>(a, wide, blocks, st);
-  else if (p->residual_dtype == TMOE_F32) launch_backward<bf16, float>(a, wide, blocks, st);
-  else launch_backward<bf16, bf16>(a, wide, blocks, st);
+  const NormShape s = norm_shape(p->d);
+  a.tw = s.tw;
+  TMOE_NORM_TYPES(launch_backward, p, a, s, wide, blocks, st);
   count_launch();
   if ((rc = launch_status())) return rc;
   if (params) {
-    const dim3 grid((unsigned)((a.n_sums * p->d + 31) / 32));
+    const int grid = (a.n_sums * p->d + 31) / 32;
     if (p->dtype == TMOE_F32)
-      norm_params_kernel<float><<<grid, 256, 0, st>>>(a.partial, blocks, a.n_sums, p->d, (float *)d_layer_scale, (float *)d_post_w,
-                                                      (float *)d_next_w, a.sum_ls, a.sum_w0, a.sum_w1);
+      norm_params_kernel<float><<<grid, 256, 0, st>>>(a, blocks, (float *)d_layer_scale, (float *)d_post_w, (float *)d_next_w);
     else
-      norm_params_kernel<bf16><<<grid, 256, 0, st>>>(a.partial, blocks, a.n_sums, p->d, (bf16 *)d_layer_scale, (bf16 *)d_post_w,
-                                                     (bf16 *)d_next_w, a.sum_ls, a.sum_w0, a.sum_w1);
+      norm_params_kernel<bf16><<<grid, 256, 0, st>>>(a, blocks, (bf16 *)d_layer_scale, (bf16 *)d_post_w, (bf16 *)d_next_w);
     count_launch();
     rc = launch_status();
   }
