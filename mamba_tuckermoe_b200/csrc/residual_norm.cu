@@ -30,7 +30,36 @@ namespace tmoe {
 namespace {
 
 constexpr int kMaxWidth = 8192;      // widest row: 512 threads x 16 elements
-constexpr int kNormThreads = 512;    // upper bound of the block size
+// Warps of a block and blocks resident on an SM, by the registers a thread needs: forward 4 x 8 warps (64 registers) or larger blocks
+// of one row each; backward one block of 20 (96 registers).  Threads with 16 elements take 16 warps (128 registers).
+constexpr int kForwardWarps = 32, kBackwardWarps = 20, kWideWarps = 16;
+constexpr int resident_warps(int nv, bool back) { return nv == 2 ? kWideWarps : back ? kBackwardWarps : kForwardWarps; }
+constexpr int max_block(int nv, bool back) { return 32 * (nv == 2 ? kWideWarps : kBackwardWarps); }
+constexpr int kRingBytes = 208 * 1024;
+
+// Two fp32 values worked on by one instruction: the walk is bound by the instructions it issues as much as by memory (80 a element in
+// scalar form), and sm_100 multiplies and adds pairs at the price of one.
+using f2 = unsigned long long;
+__device__ __forceinline__ f2 pair(float lo, float hi) { f2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi)); return r; }
+__device__ __forceinline__ f2 both(float v) { return pair(v, v); }
+__device__ __forceinline__ void split(f2 v, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) { f2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ f2 add2(f2 a, f2 b) { f2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) { f2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+__device__ __forceinline__ float sum2(f2 v) { float a, b; split(v, a, b); return a + b; }
+
+// sigmoid to a few ulp (the gate is one factor of a sum that is rounded to the storage type).  exp(-g) beyond the range is 0 or infinite,
+// and its reciprocal 1 or 0.
+__device__ __forceinline__ f2 sigmoid2(f2 g) {
+  float a, b;
+  split(mul2(g, both(-1.4426950408889634f)), a, b);
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(a));
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(b));
+  split(add2(pair(a, b), both(1.f)), a, b);
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(a));
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(b));
+  return pair(a, b);
+}
 
 __device__ __forceinline__ void cp_async16(void *smem, const void *gmem) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ptx::smem_u32(smem)), "l"(gmem) : "memory");
@@ -49,13 +78,13 @@ template <> struct Piece<bf16, 8> {
   __device__ __forceinline__ void load(const bf16 *p) { r = *reinterpret_cast<const uint4 *>(p); }
   __device__ __forceinline__ void zero() { r = make_uint4(0, 0, 0, 0); }
   __device__ __forceinline__ void one() { r = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u); }
-  __device__ __forceinline__ float get(int q) const {
-    const uint32_t w = (q >> 1) == 0 ? r.x : (q >> 1) == 1 ? r.y : (q >> 1) == 2 ? r.z : r.w;
-    return __uint_as_float((q & 1) ? (w & 0xffff0000u) : (w << 16));
+  __device__ __forceinline__ f2 get2(int j) const {   // elements 2j, 2j + 1
+    const uint32_t w = j == 0 ? r.x : j == 1 ? r.y : j == 2 ? r.z : r.w;
+    return pair(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
   }
-  __device__ static __forceinline__ void store(bf16 *p, const float (&f)[8]) {
-    *reinterpret_cast<uint4 *>(p) =
-        make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+  __device__ static __forceinline__ uint32_t pack(f2 v) { float a, b; split(v, a, b); return pack_bf16x2(a, b); }
+  __device__ static __forceinline__ void store(bf16 *p, const f2 *f) {
+    *reinterpret_cast<uint4 *>(p) = make_uint4(pack(f[0]), pack(f[1]), pack(f[2]), pack(f[3]));
   }
 };
 template <> struct Piece<float, 8> {
@@ -72,13 +101,13 @@ template <> struct Piece<float, 8> {
   }
   __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
   __device__ __forceinline__ void one() { a = b = make_float4(1.f, 1.f, 1.f, 1.f); }
-  __device__ __forceinline__ float get(int q) const {
-    const float4 v = q < 4 ? a : b;
-    return (q & 3) == 0 ? v.x : (q & 3) == 1 ? v.y : (q & 3) == 2 ? v.z : v.w;
+  __device__ __forceinline__ f2 get2(int j) const {
+    const float4 v = j < 2 ? a : b;
+    return (j & 1) ? pair(v.z, v.w) : pair(v.x, v.y);
   }
-  __device__ static __forceinline__ void store(float *p, const float (&f)[8]) {
-    reinterpret_cast<float4 *>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
-    reinterpret_cast<float4 *>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+  __device__ static __forceinline__ void store(float *p, const f2 *f) {
+    reinterpret_cast<ulonglong2 *>(p)[0] = make_ulonglong2(f[0], f[1]);
+    reinterpret_cast<ulonglong2 *>(p)[1] = make_ulonglong2(f[2], f[3]);
   }
 };
 template <typename T> struct Piece<T, 1> {
@@ -89,9 +118,29 @@ template <typename T> struct Piece<T, 1> {
   __device__ __forceinline__ void load(const T *p) { r = *p; }
   __device__ __forceinline__ void zero() { r = from_f32<T>(0.f); }
   __device__ __forceinline__ void one() { r = from_f32<T>(1.f); }
-  __device__ __forceinline__ float get(int) const { return to_f32(r); }
-  __device__ static __forceinline__ void store(T *p, const float (&f)[1]) { *p = from_f32<T>(f[0]); }
+  __device__ __forceinline__ float get() const { return to_f32(r); }
 };
+
+// Pairs over a thread's NV * VEC elements: neighbours in a piece, or two pieces where a piece is one element.
+template <typename T, int NV> __device__ __forceinline__ f2 pair_of(const Piece<T, 8> (&p)[NV], int j) { return p[j / 4].get2(j % 4); }
+template <typename T, int NV> __device__ __forceinline__ f2 pair_of(const Piece<T, 1> (&p)[NV], int j) { return pair(p[2 * j].get(), p[2 * j + 1].get()); }
+// Stores a thread's pairs to columns (i * tpr + lt) * VEC ... of one row of width d.
+template <typename T, int VEC, int NV>
+__device__ __forceinline__ void store_row(T *row, int tpr, int lt, int d, const f2 (&f)[NV * VEC / 2]) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int e = (i * tpr + lt) * VEC;
+    if (e < d) {
+      if constexpr (VEC == 8) {
+        Piece<T, 8>::store(row + e, f + i * 4);
+      } else {
+        float a, b;
+        split(f[i / 2], a, b);
+        row[e] = from_f32<T>((i & 1) ? b : a);
+      }
+    }
+  }
+}
 
 struct NormArgs {
   const void *y, *res, *ls, *gate, *w0, *w1;  // inputs; nullptr = the term is absent
@@ -110,16 +159,16 @@ struct NormArgs {
   int n_sums;
 };
 
-// Sums over the `tw` warps of a team, in a fixed order.  A team has 16 places of shared memory for each sum, zero beyond its own warps
+// Sums over the `tw` warps of a team, in a fixed order.  A team has 20 places of shared memory for each sum, zero beyond its own warps
 // (TeamRed::init), which every thread reads back with wide loads; `slot` alternates between calls, so one barrier per call is enough.
 template <int N> struct TeamRed {
-  float at[2][8][N][16];   // [slot][team][sum][warp]
+  float at[2][10][N][20];   // [slot][team][sum][warp]
   __device__ __forceinline__ void init() {
-    for (int i = threadIdx.x; i < 2 * 8 * N * 16; i += blockDim.x) (&at[0][0][0][0])[i] = 0.f;
+    for (int i = threadIdx.x; i < 2 * 10 * N * 20; i += blockDim.x) (&at[0][0][0][0])[i] = 0.f;
     __syncthreads();
   }
 };
-__device__ __forceinline__ float sum_places(const float (&v)[16], int tw) {
+__device__ __forceinline__ float sum_places(const float (&v)[20], int tw) {
   const float4 *p = reinterpret_cast<const float4 *>(v);
   const float4 a = p[0];
   float s = (a.x + a.y) + (a.z + a.w);
@@ -129,6 +178,10 @@ __device__ __forceinline__ float sum_places(const float (&v)[16], int tw) {
     if (tw > 8) {
       const float4 c = p[2], d = p[3];
       s += ((c.x + c.y) + (c.z + c.w)) + ((d.x + d.y) + (d.z + d.w));
+      if (tw > 16) {
+        const float4 e = p[4];
+        s += (e.x + e.y) + (e.z + e.w);
+      }
     }
   }
   return s;
@@ -159,127 +212,162 @@ __device__ __forceinline__ float3 team_sum3(float a, float b, float c, int tw, i
   return make_float3(sum_places(red.at[slot][team][0], tw), sum_places(red.at[slot][team][1], tw), sum_places(red.at[slot][team][2], tw));
 }
 
-// exp and reciprocal to a few ulp: the gate is one factor of a sum that is rounded to the storage type
-__device__ __forceinline__ float sigmoid(float g) { return __fdividef(1.f, 1.f + __expf(-g)); }
+extern __shared__ uint4 norm_ring[];
 
-// One row's inputs as they lie in memory.  Where the ring has stages, a row's pieces are copied to shared memory some rows ahead; a
-// thread copies and reads its own pieces only, so the ring needs no barrier, just the thread's own wait for its copies.
+// One row's inputs as they lie in memory, and the walk of a team over its rows.  Where the ring has stages, a row's pieces are copied to
+// shared memory some rows ahead; a thread copies and reads its own pieces only, so the ring needs no barrier, just the thread's own
+// wait for its copies.  What is never copied (an absent operand, a column beyond the row) is zero in the ring from the start, so reading
+// needs no conditions.
 template <typename TY, typename TR, int VEC, int NV, bool GATE, bool BACK> struct RowIn {
   using PY = Piece<TY, VEC>;
   using PR = Piece<TR, VEC>;
   static constexpr int kPlanes = NV * ((1 + (GATE ? 1 : 0) + (BACK ? 1 : 0)) * PY::kPlanes + (BACK ? 2 : 1) * PR::kPlanes);
-  // as many rows ahead as 192 KB hold for the warps that an SM is meant to run; below 2 stages rows are loaded when their turn comes
-  static constexpr int kWarps = BACK || NV == 2 ? 16 : 32;
-  static constexpr int kFit = kPlanes ? 196608 / (kPlanes * kWarps * 512) : 0;
+  // as many rows ahead as fit for the warps that an SM is meant to run; below 2 stages rows are loaded when their turn comes
+  // (backward, the parameters' columns of a thread lie behind the ring, in fp32)
+  static constexpr int kParamPlanes = BACK && VEC == 8 ? 4 * NV : 0;
+  static constexpr int kFit = kPlanes ? (kRingBytes / (resident_warps(NV, BACK) * 512) - kParamPlanes) / kPlanes : 0;
   static constexpr int kStages = kFit >= 3 ? 3 : kFit == 2 ? 2 : 1;
   static constexpr bool kRing = kStages > 1;
   PY y[NV], g[GATE ? NV : 1], dn[BACK ? NV : 1];
   PR r[NV], dout[BACK ? NV : 1];
-
-  __device__ static __forceinline__ void copy(const NormArgs &a, int64_t row, int tpr, int lt, uint4 *slot, int pitch) {
-    if (row < a.rows) {
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int e = (i * tpr + lt) * VEC;
-        if (e < a.d) {
-          PY::copy(slot, pitch, (const TY *)a.y + row * a.ys + e);
-          slot += PY::kPlanes * pitch;
-          if (GATE) { PY::copy(slot, pitch, (const TY *)a.gate + row * a.gs + e); slot += PY::kPlanes * pitch; }
-          if (BACK) { if (a.d_normed) PY::copy(slot, pitch, (const TY *)a.d_normed + row * a.dns + e); slot += PY::kPlanes * pitch; }
-          if (a.res) PR::copy(slot, pitch, (const TR *)a.res + row * a.rs + e);
-          slot += PR::kPlanes * pitch;
-          if (BACK) { if (a.d_out) PR::copy(slot, pitch, (const TR *)a.d_out + row * a.dos + e); slot += PR::kPlanes * pitch; }
-        }
-      }
-    }
-    cp_async_commit();
-  }
-  __device__ __forceinline__ void fetch(const NormArgs &a, int tpr, int lt, const uint4 *slot, int pitch) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      y[i].zero(); r[i].zero();
-      if (GATE) g[i].zero();
-      if (BACK) { dn[i].zero(); dout[i].zero(); }
-      if ((i * tpr + lt) * VEC < a.d) {
-        y[i].fetch(slot, pitch);
-        slot += PY::kPlanes * pitch;
-        if (GATE) { g[i].fetch(slot, pitch); slot += PY::kPlanes * pitch; }
-        if (BACK) { if (a.d_normed) dn[i].fetch(slot, pitch); slot += PY::kPlanes * pitch; }
-        if (a.res) r[i].fetch(slot, pitch);
-        slot += PR::kPlanes * pitch;
-        if (BACK) { if (a.d_out) dout[i].fetch(slot, pitch); slot += PR::kPlanes * pitch; }
-      }
-    }
-  }
-  __device__ __forceinline__ void load(const NormArgs &a, int64_t row, int tpr, int lt) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int e = (i * tpr + lt) * VEC;
-      y[i].zero(); r[i].zero();
-      if (GATE) g[i].zero();
-      if (BACK) { dn[i].zero(); dout[i].zero(); }
-      if (e < a.d) {
-        y[i].load((const TY *)a.y + row * a.ys + e);
-        if (a.res) r[i].load((const TR *)a.res + row * a.rs + e);
-        if (GATE) g[i].load((const TY *)a.gate + row * a.gs + e);
-        if (BACK) {
-          if (a.d_out) dout[i].load((const TR *)a.d_out + row * a.dos + e);
-          if (a.d_normed) dn[i].load((const TY *)a.d_normed + row * a.dns + e);
-        }
-      }
-    }
-  }
 };
 
-// The rows of one team, one after the other.
-template <typename In> struct RowWalk {
+template <typename TY, typename TR, int VEC, int NV, bool GATE, bool BACK> struct RowWalk {
+  using In = RowIn<TY, TR, VEC, NV, GATE, BACK>;
+  using PY = Piece<TY, VEC>;
+  using PR = Piece<TR, VEC>;
+  // this thread's first piece in the row that is copied (or, without a ring, loaded) next
+  const TY *y, *g, *dn;
+  const TR *r, *o;
+  int64_t ahead;       // that row
   uint4 *slot;
-  int64_t step;
   int stage;
-  __device__ __forceinline__ RowWalk(const NormArgs &a, int64_t row, int64_t step_, uint4 *ring, int tpr, int lt)
-      : slot(ring + threadIdx.x), step(step_), stage(0) {
+
+  __device__ __forceinline__ RowWalk(const NormArgs &a, int64_t row, int64_t step, int lt) : ahead(row), slot(norm_ring + threadIdx.x), stage(0) {
+    y = (const TY *)a.y + row * a.ys + lt * VEC;
+    g = (const TY *)a.gate + row * a.gs + lt * VEC;
+    dn = (const TY *)a.d_normed + row * a.dns + lt * VEC;
+    r = (const TR *)a.res + row * a.rs + lt * VEC;
+    o = (const TR *)a.d_out + row * a.dos + lt * VEC;
     if (In::kRing) {
 #pragma unroll
-      for (int s = 0; s < In::kStages - 1; ++s) In::copy(a, row + s * step, tpr, lt, at(s), blockDim.x);
+      for (int i = 0; i < In::kStages * In::kPlanes; ++i) slot[i * blockDim.x] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int s = 0; s < In::kStages - 1; ++s) copy(a, step, lt, at(s));
     }
   }
   __device__ __forceinline__ uint4 *at(int s) const { return slot + s * In::kPlanes * blockDim.x; }
-  __device__ __forceinline__ void take(const NormArgs &a, int64_t row, int tpr, int lt, In &in) {
-    if (In::kRing) {
-      const int last = stage == 0 ? In::kStages - 1 : stage - 1;
-      In::copy(a, row + (In::kStages - 1) * step, tpr, lt, at(last), blockDim.x);
-      cp_async_wait<In::kStages - 1>();
-      in.fetch(a, tpr, lt, at(stage), blockDim.x);
-      stage = stage + 1 == In::kStages ? 0 : stage + 1;
-    } else {
-      in.load(a, row, tpr, lt);
-    }
+  __device__ __forceinline__ uint4 *behind() const { return at(In::kStages); }
+  __device__ __forceinline__ void advance(const NormArgs &a, int64_t step) {
+    ahead += step;
+    y += step * a.ys;
+    r += step * a.rs;
+    if (GATE) g += step * a.gs;
+    if (BACK) { dn += step * a.dns; o += step * a.dos; }
   }
-};
-
-// The parameter vectors' columns of one thread (1 where a factor is absent).  With 8 columns a thread they stay in registers over all
-// its rows; with 16 they are read again (from L1) for each, which is cheaper than the spills they cause.
-template <typename TY, int VEC, int NV> struct Params {
-  Piece<TY, VEC> w0[NV], ls[NV], w1[NV];
-  __device__ __forceinline__ void load(const NormArgs &a, int tpr, int lt) {
+  __device__ __forceinline__ void copy(const NormArgs &a, int64_t step, int lt, uint4 *to) {
+    if (ahead < a.rows) {
+      const int pitch = blockDim.x, tpr = a.tw * 32;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int e = (i * tpr + lt) * VEC;
-      w0[i].zero(); ls[i].zero(); w1[i].zero();
-      if (e < a.d) {
-        if (a.w0) w0[i].load((const TY *)a.w0 + e); else w0[i].one();
-        if (a.ls) ls[i].load((const TY *)a.ls + e); else ls[i].one();
-        if (a.w1) w1[i].load((const TY *)a.w1 + e);
+      for (int i = 0; i < NV; ++i) {
+        const int e = i * tpr * VEC;
+        if (lt * VEC + e < a.d) {
+          PY::copy(to, pitch, y + e);
+          if (GATE) PY::copy(to + PY::kPlanes * pitch, pitch, g + e);
+          if (a.res) PR::copy(to + kR * pitch, pitch, r + e);
+          if (BACK && a.d_normed) PY::copy(to + kN * pitch, pitch, dn + e);
+          if (BACK && a.d_out) PR::copy(to + kO * pitch, pitch, o + e);
+        }
+        to += In::kPlanes / NV * pitch;
       }
     }
+    advance(a, step);
+    cp_async_commit();
   }
+  // planes of one piece: y, gate, residual, d_normed, d_out
+  static constexpr int kR = (GATE ? 2 : 1) * PY::kPlanes, kN = kR + PR::kPlanes, kO = kN + PY::kPlanes;
+  __device__ __forceinline__ void fetch(const uint4 *from, In &in) const {
+    const int pitch = blockDim.x;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      in.y[i].fetch(from, pitch);
+      if (GATE) in.g[i].fetch(from + PY::kPlanes * pitch, pitch);
+      in.r[i].fetch(from + kR * pitch, pitch);
+      if (BACK) { in.dn[i].fetch(from + kN * pitch, pitch); in.dout[i].fetch(from + kO * pitch, pitch); }
+      from += In::kPlanes / NV * pitch;
+    }
+  }
+  __device__ __forceinline__ void take(const NormArgs &a, int64_t step, int lt, In &in) {
+    if (In::kRing) {
+      copy(a, step, lt, at(stage == 0 ? In::kStages - 1 : stage - 1));
+      cp_async_wait<In::kStages - 1>();
+      fetch(at(stage), in);
+      stage = stage + 1 == In::kStages ? 0 : stage + 1;
+    } else {
+      const int tpr = a.tw * 32;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int e = i * tpr * VEC;
+        in.y[i].zero(); in.r[i].zero();
+        if (GATE) in.g[i].zero();
+        if (BACK) { in.dn[i].zero(); in.dout[i].zero(); }
+        if (lt * VEC + e < a.d) {
+          in.y[i].load(y + e);
+          if (a.res) in.r[i].load(r + e);
+          if (GATE) in.g[i].load(g + e);
+          if (BACK) {
+            if (a.d_out) in.dout[i].load(o + e);
+            if (a.d_normed) in.dn[i].load(dn + e);
+          }
+        }
+      }
+      advance(a, step);
+    }
+  }
+  // the row taken last, once more
+  __device__ __forceinline__ void again(In &in) const { fetch(at(stage == 0 ? In::kStages - 1 : stage - 1), in); }
 };
 
-extern __shared__ uint4 norm_ring[];
+// The parameter vectors' columns of one thread (1 where a factor is absent): c = post_w * layer_scale, w1 = next_w.
+template <typename TY, int VEC, int NV> struct Params {
+  static constexpr int N2 = NV * VEC / 2;
+  f2 c[N2], w1[N2];
+  __device__ __forceinline__ void load(const NormArgs &a, int lt) {
+    Piece<TY, VEC> p0[NV], pl[NV], p1[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int e = (i * a.tw * 32 + lt) * VEC;
+      p0[i].zero(); pl[i].zero(); p1[i].zero();
+      if (e < a.d) {
+        if (a.w0) p0[i].load((const TY *)a.w0 + e); else p0[i].one();
+        if (a.ls) pl[i].load((const TY *)a.ls + e); else pl[i].one();
+        if (a.w1) p1[i].load((const TY *)a.w1 + e);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < N2; ++j) { c[j] = mul2(pair_of(p0, j), pair_of(pl, j)); w1[j] = pair_of(p1, j); }
+  }
+  // 16-byte parts: c first, then w1
+  __device__ __forceinline__ void keep(uint4 *slot) const {
+#pragma unroll
+    for (int j = 0; j < N2; j += 2) {
+      *reinterpret_cast<ulonglong2 *>(slot + j / 2 * blockDim.x) = make_ulonglong2(c[j], c[j + 1]);
+      *reinterpret_cast<ulonglong2 *>(slot + (N2 / 2 + j / 2) * blockDim.x) = make_ulonglong2(w1[j], w1[j + 1]);
+    }
+  }
+  __device__ __forceinline__ void fetch(const uint4 *slot) {
+#pragma unroll
+    for (int j = 0; j < N2; j += 2) {
+      const ulonglong2 p = *reinterpret_cast<const ulonglong2 *>(slot + j / 2 * blockDim.x);
+      const ulonglong2 q = *reinterpret_cast<const ulonglong2 *>(slot + (N2 / 2 + j / 2) * blockDim.x);
+      c[j] = p.x; c[j + 1] = p.y; w1[j] = q.x; w1[j + 1] = q.y;
+    }
+  }
+};
 
 // A team walks over rows blockIdx * teams + team, + gridDim * teams, ...
 template <typename TY, typename TR, int VEC, int NV, bool GATE>
-__global__ void __launch_bounds__(kNormThreads, NV == 1 && VEC == 8 ? 2 : 1) residual_norm_kernel(const __grid_constant__ NormArgs a) {
+__global__ void __launch_bounds__(VEC == 8 && NV == 1 ? 512 : max_block(VEC == 8 ? NV : NV / 8, false), VEC == 8 && NV == 1 ? 2 : 1) residual_norm_kernel(const __grid_constant__ NormArgs a) {
   using In = RowIn<TY, TR, VEC, NV, GATE, false>;
   __shared__ __align__(16) TeamRed<1> red;
   red.init();
@@ -287,52 +375,39 @@ __global__ void __launch_bounds__(kNormThreads, NV == 1 && VEC == 8 ? 2 : 1) res
   const int64_t step = (int64_t)gridDim.x * (blockDim.x / tpr);
   int64_t row = (int64_t)blockIdx.x * (blockDim.x / tpr) + team;
   const float inv_d = 1.f / (float)a.d;
-  RowWalk<In> walk(a, row, step, norm_ring, tpr, lt);
+  RowWalk<TY, TR, VEC, NV, GATE, false> walk(a, row, step, lt);
   Params<TY, VEC, NV> w;
-  w.load(a, tpr, lt);
+  w.load(a, lt);
   int slot = 0;
   for (; row < a.rows; row += step) {
     In in;
-    walk.take(a, row, tpr, lt, in);
+    walk.take(a, step, lt, in);
+    constexpr int N2 = NV * VEC / 2;
     float rho0 = 1.f;
     if (a.w0) {
-      float ss = 0.f;
+      f2 ss = both(0.f);
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-#pragma unroll
-        for (int q = 0; q < VEC; ++q) ss = fmaf(in.y[i].get(q), in.y[i].get(q), ss);
-      }
-      ss = team_sum(ss, a.tw, team, slot, red);
+      for (int j = 0; j < N2; ++j) ss = fma2(pair_of(in.y, j), pair_of(in.y, j), ss);
+      rho0 = rsqrtf(fmaf(team_sum(sum2(ss), a.tw, team, slot, red), inv_d, a.eps0));
       slot ^= 1;
-      rho0 = rsqrtf(fmaf(ss, inv_d, a.eps0));
       if (a.rstd && lt == 0) a.rstd[row] = rho0;
     }
-    float v[NV][VEC], ss = 0.f;
+    f2 v[N2], ss = both(0.f);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-#pragma unroll
-      for (int q = 0; q < VEC; ++q) {
-        float t = in.y[i].get(q) * rho0 * w.w0[i].get(q);
-        if (GATE) { const float g = in.g[i].get(q); t *= g * sigmoid(g); }
-        t = fmaf(t, w.ls[i].get(q), in.r[i].get(q));
-        v[i][q] = t;
-        ss = fmaf(t, t, ss);
-      }
-      const int e = (i * tpr + lt) * VEC;
-      if (a.out && e < a.d) Piece<TR, VEC>::store((TR *)a.out + row * a.d + e, v[i]);
+    for (int j = 0; j < N2; ++j) {
+      f2 t = mul2(mul2(pair_of(in.y, j), both(rho0)), w.c[j]);
+      if (GATE) { const f2 g = pair_of(in.g, j); t = mul2(t, mul2(g, sigmoid2(g))); }
+      v[j] = add2(t, pair_of(in.r, j));
+      ss = fma2(v[j], v[j], ss);
     }
+    if (a.out) store_row<TR, VEC, NV>((TR *)a.out + row * a.d, tpr, lt, a.d, v);
     if (!a.normed) continue;
-    ss = team_sum(ss, a.tw, team, slot, red);
+    const float rho1 = rsqrtf(fmaf(team_sum(sum2(ss), a.tw, team, slot, red), inv_d, a.eps1));
     slot ^= 1;
-    const float rho1 = rsqrtf(fmaf(ss, inv_d, a.eps1));
     if (a.rstd && lt == 0) a.rstd[a.rows + row] = rho1;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int e = (i * tpr + lt) * VEC;
-#pragma unroll
-      for (int q = 0; q < VEC; ++q) v[i][q] *= rho1 * w.w1[i].get(q);
-      if (e < a.d) Piece<TY, VEC>::store((TY *)a.normed + row * a.d + e, v[i]);
-    }
+    for (int j = 0; j < N2; ++j) v[j] = mul2(v[j], mul2(both(rho1), w.w1[j]));
+    store_row<TY, VEC, NV>((TY *)a.normed + row * a.d, tpr, lt, a.d, v);
   }
 }
 
@@ -341,7 +416,7 @@ __global__ void __launch_bounds__(kNormThreads, NV == 1 && VEC == 8 ? 2 : 1) res
 // adds its teams in order and writes one row of partial sums; norm_params_kernel adds the blocks in order.  The result depends on the
 // sizes and the grid only.
 template <typename TY, typename TR, int VEC, int NV, bool GATE>
-__global__ void __launch_bounds__(kNormThreads) residual_norm_backward_kernel(const __grid_constant__ NormArgs a) {
+__global__ void __launch_bounds__(max_block(VEC == 8 ? NV : NV / 8, true)) residual_norm_backward_kernel(const __grid_constant__ NormArgs a) {
   using In = RowIn<TY, TR, VEC, NV, GATE, true>;
   __shared__ __align__(16) TeamRed<3> red;
   red.init();
@@ -349,16 +424,16 @@ __global__ void __launch_bounds__(kNormThreads) residual_norm_backward_kernel(co
   const int64_t step = (int64_t)gridDim.x * teams;
   int64_t row = (int64_t)blockIdx.x * teams + team;
   const float inv_d = 1.f / (float)a.d;
-  RowWalk<In> walk(a, row, step, norm_ring, tpr, lt);
-  constexpr bool kKeep = NV * VEC <= 8;
+  RowWalk<TY, TR, VEC, NV, GATE, true> walk(a, row, step, lt);
+  // Registers are what decides how many rows an SM works on.  With a ring a thread reads its pieces of the row and of the parameters
+  // from shared memory in both passes over the row, so that only x, b and the sums stay in registers across the reduction.
   Params<TY, VEC, NV> w;
-  w.load(a, tpr, lt);
-  float acc_a[NV][VEC], acc_x[NV][VEC];
+  w.load(a, lt);
+  if (In::kRing) w.keep(walk.behind());
+  constexpr int N2 = NV * VEC / 2;
+  f2 acc_a[N2], acc_x[N2];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-#pragma unroll
-    for (int q = 0; q < VEC; ++q) acc_a[i][q] = acc_x[i][q] = 0.f;
-  }
+  for (int j = 0; j < N2; ++j) acc_a[j] = acc_x[j] = both(0.f);
   int slot = 0;
   // without dN nothing flows through the next norm; one row's rstd are loaded a row ahead
   float next0 = a.w0 && row < a.rows ? a.rstd[row] : 1.f, next1 = a.d_normed && row < a.rows ? a.rstd[a.rows + row] : 0.f;
@@ -369,58 +444,58 @@ __global__ void __launch_bounds__(kNormThreads) residual_norm_backward_kernel(co
       if (a.d_normed) next1 = a.rstd[a.rows + row + step];
     }
     In in;
-    walk.take(a, row, tpr, lt, in);
-    if (!kKeep) w.load(a, tpr, lt);
-    float x[NV][VEC], b[NV][VEC], s1 = 0.f, s2 = 0.f, s3 = 0.f;   // sum u*x, sum q*b, sum q*x
+    walk.take(a, step, lt, in);
+    if (In::kRing) w.fetch(walk.behind());
+    f2 x[N2], b[N2], s1 = both(0.f), s2 = s1, s3 = s1;   // sum u*x, sum q*b, sum q*x
+    const f2 r0 = both(rho0), r1 = both(rho1);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-#pragma unroll
-      for (int q = 0; q < VEC; ++q) {
-        float t = in.y[i].get(q) * rho0 * w.w0[i].get(q) * w.ls[i].get(q);
-        if (GATE) { const float g = in.g[i].get(q); t *= g * sigmoid(g); }
-        x[i][q] = (in.r[i].get(q) + t) * rho1;
-        const float u = w.w1[i].get(q) * in.dn[i].get(q);
-        b[i][q] = fmaf(rho1, u, in.dout[i].get(q));
-        s1 = fmaf(u, x[i][q], s1);
-        s2 = fmaf(t, b[i][q], s2);
-        s3 = fmaf(t, x[i][q], s3);
-      }
+    for (int j = 0; j < N2; ++j) {
+      f2 t = mul2(mul2(pair_of(in.y, j), r0), w.c[j]);
+      if (GATE) { const f2 g = pair_of(in.g, j); t = mul2(t, mul2(g, sigmoid2(g))); }
+      x[j] = mul2(add2(pair_of(in.r, j), t), r1);
+      const f2 u = mul2(w.w1[j], pair_of(in.dn, j));
+      b[j] = fma2(r1, u, pair_of(in.dout, j));
+      s1 = fma2(u, x[j], s1);
+      s2 = fma2(t, b[j], s2);
+      s3 = fma2(t, x[j], s3);
     }
     float k1 = 0.f, k0 = 0.f;
     if (a.w0 || a.d_normed) {
-      const float3 r = team_sum3(s1, s2, s3, a.tw, team, slot, red);
+      const float3 r = team_sum3(sum2(s1), sum2(s2), sum2(s3), a.tw, team, slot, red);
       slot ^= 1;
       k1 = rho1 * r.x * inv_d;
       k0 = a.w0 ? rho0 * inv_d * (r.y - k1 * r.z) : 0.f;
     }
-    if (!kKeep) w.load(a, tpr, lt);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int e = (i * tpr + lt) * VEC;
-      float f[VEC];
-#pragma unroll
-      for (int q = 0; q < VEC; ++q) {
-        b[i][q] = fmaf(-k1, x[i][q], b[i][q]);                        // dR
-        acc_x[i][q] = fmaf(in.dn[i].get(q), x[i][q], acc_x[i][q]);
-      }
-      if (a.d_res && e < a.d) Piece<TR, VEC>::store((TR *)a.d_res + row * a.d + e, b[i]);
-      if (GATE) {
-#pragma unroll
-        for (int q = 0; q < VEC; ++q) {
-          const float g = in.g[i].get(q), sg = sigmoid(g), h = in.y[i].get(q) * rho0;
-          f[q] = b[i][q] * w.ls[i].get(q) * w.w0[i].get(q) * h * (sg * fmaf(g, 1.f - sg, 1.f));
-          b[i][q] *= g * sg;                                           // dR * s
-        }
-        if (a.d_gate && e < a.d) Piece<TY, VEC>::store((TY *)a.d_gate + row * a.d + e, f);
-      }
-#pragma unroll
-      for (int q = 0; q < VEC; ++q) {
-        const float h = in.y[i].get(q) * rho0;
-        acc_a[i][q] = fmaf(b[i][q], h, acc_a[i][q]);
-        f[q] = fmaf(b[i][q] * rho0, w.w0[i].get(q) * w.ls[i].get(q), -k0 * h);
-      }
-      if (a.d_y && e < a.d) Piece<TY, VEC>::store((TY *)a.d_y + row * a.d + e, f);
+    if (In::kRing) {
+      walk.again(in);
+      w.fetch(walk.behind());
     }
+    const f2 n1 = both(-k1), n0 = both(-k0);
+#pragma unroll
+    for (int j = 0; j < N2; ++j) {
+      b[j] = fma2(n1, x[j], b[j]);                                     // dR
+      acc_x[j] = fma2(pair_of(in.dn, j), x[j], acc_x[j]);
+    }
+    if (a.d_res) store_row<TR, VEC, NV>((TR *)a.d_res + row * a.d, tpr, lt, a.d, b);
+    if (GATE) {
+      f2 f[N2];
+#pragma unroll
+      for (int j = 0; j < N2; ++j) {
+        const f2 g = pair_of(in.g, j), sg = sigmoid2(g), s = mul2(g, sg);
+        const f2 ch = mul2(mul2(pair_of(in.y, j), r0), w.c[j]);
+        // silu'(g) = sg + silu(g) * (1 - sg)
+        f[j] = mul2(mul2(b[j], ch), fma2(s, fma2(sg, both(-1.f), both(1.f)), sg));
+        b[j] = mul2(b[j], s);                                          // dR * s
+      }
+      if (a.d_gate) store_row<TY, VEC, NV>((TY *)a.d_gate + row * a.d, tpr, lt, a.d, f);
+    }
+#pragma unroll
+    for (int j = 0; j < N2; ++j) {
+      const f2 h = mul2(pair_of(in.y, j), r0);
+      acc_a[j] = fma2(b[j], h, acc_a[j]);
+      b[j] = fma2(mul2(b[j], r0), w.c[j], mul2(n0, h));
+    }
+    if (a.d_y) store_row<TY, VEC, NV>((TY *)a.d_y + row * a.d, tpr, lt, a.d, b);
   }
   if (!a.partial) return;
   // [d] floats where the ring was, when a block has several teams: all of its copies have landed and been read by then
@@ -440,7 +515,10 @@ __global__ void __launch_bounds__(kNormThreads) residual_norm_backward_kernel(co
           if (e < a.d) {
 #pragma unroll
             for (int q = 0; q < VEC; ++q) {
-              float t = k == 0 ? acc_a[i][q] : acc_x[i][q];
+              const int n = i * VEC + q;
+              float lo, hi;
+              split(k == 0 ? acc_a[n / 2] : acc_x[n / 2], lo, hi);
+              float t = (n & 1) ? hi : lo;
               if (m > 0) t += fold[e + q];
               if (m == teams - 1) dst[(int64_t)at * a.d + e + q] = t;
               else fold[e + q] = t;
@@ -478,16 +556,23 @@ __global__ void __launch_bounds__(256) norm_params_kernel(const __grid_constant_
   }
 }
 
-struct NormShape { int tw, nv, teams; };
+struct NormShape { int tw, nv, teams, blocks; };
 
-// Warps per row, pieces per thread, rows worked on at once by a block.  One 8-element piece per thread up to 4096 columns: a row
-// spread over several warps costs a barrier, but leaves registers for the next row's loads and enough warps on an SM.
-NormShape norm_shape(int d) {
+// Warps per row, pieces per thread, rows worked on at once by a block, blocks.  One 8-element piece per thread where a row's warps then
+// fit a block: a row spread over several warps costs a barrier, but leaves registers and shared memory for the rows ahead.  Few rows are
+// spread over the SMs before a block takes several.
+NormShape norm_shape(int64_t rows, int d, bool back, int sms) {
   NormShape s;
   const int pieces = (d + 7) / 8;
-  s.nv = pieces <= 512 ? 1 : 2;
+  s.nv = pieces <= 32 * (back ? kBackwardWarps : kWideWarps) ? 1 : 2;
   s.tw = (pieces + 32 * s.nv - 1) / (32 * s.nv);
-  s.teams = s.tw >= 8 ? 1 : 8 / s.tw;
+  const int resident = resident_warps(s.nv, back), full = back ? resident : 8;
+  s.teams = s.tw >= full ? 1 : full / s.tw;
+  if (s.tw > 1 && s.teams > 10) s.teams = 10;
+  const int64_t each = (rows + sms - 1) / sms;
+  if (each < s.teams) s.teams = each < 1 ? 1 : (int)each;
+  const int64_t want = (rows + s.teams - 1) / s.teams, cap = (int64_t)sms * (back ? 1 : resident / (s.tw * s.teams) > 0 ? resident / (s.tw * s.teams) : 1);
+  s.blocks = (int)(want < cap ? want : cap);
   return s;
 }
 
@@ -530,45 +615,36 @@ bool norm_wide(const tmoe_residual_norm_t &p) {
          wide_ok(p.next_w, 0, sy);
 }
 
-// Blocks of the walk: as many as are resident at once (32 warps an SM forward, 16 backward), no more than there are rows for
-int norm_blocks(int64_t rows, int d, bool back, int sms) {
-  const NormShape s = norm_shape(d);
-  const int warps = s.tw * s.teams, resident = back || s.nv == 2 ? 16 : 32;
-  const int64_t want = (rows + s.teams - 1) / s.teams, cap = (int64_t)sms * (resident / warps);
-  return (int)(want < cap ? want : cap);
-}
-
-// Launch with `smem` bytes of dynamic shared memory; the opt-in above 48 KB (static part included) is made once per
-// kernel and device
+// Launch with the ring's shared memory; its size (and that the SM should be split for it: without that fewer blocks are resident
+// than the grid counts on) is declared once per kernel and device
 template <typename In, typename Kernel>
-void launch_walk(Kernel kernel, const NormArgs &a, const NormShape &s, int blocks, bool fold, cudaStream_t st) {
+void launch_walk(Kernel kernel, const NormArgs &a, const NormShape &s, bool fold, cudaStream_t st) {
   static std::atomic<uint64_t> opted{0};
   const int threads = s.teams * s.tw * 32;
-  size_t smem = In::kRing ? (size_t)In::kStages * In::kPlanes * threads * 16 : 0;
+  size_t smem = In::kRing ? (size_t)(In::kStages * In::kPlanes + In::kParamPlanes) * threads * 16 : 0;
   if (fold && s.teams > 1 && smem < (size_t)a.d * 4) smem = (size_t)a.d * 4;
-  if (smem > 46 * 1024) {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return;
-    const uint64_t bit = 1ull << (dev & 63);
-    if (!(opted.load(std::memory_order_relaxed) & bit)) {
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
-      opted.fetch_or(bit, std::memory_order_relaxed);
-    }
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (In::kRing && !(opted.load(std::memory_order_relaxed) & bit)) {
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
+    cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    opted.fetch_or(bit, std::memory_order_relaxed);
   }
-  kernel<<<blocks, threads, smem, st>>>(a);
+  kernel<<<s.blocks, threads, smem, st>>>(a);
 }
 
 template <typename TY, typename TR, bool GATE>
-void launch_forward(const NormArgs &a, const NormShape &s, bool wide, int blocks, cudaStream_t st) {
-#define TMOE_RN(V, N) launch_walk<RowIn<TY, TR, V, N, GATE, false>>(residual_norm_kernel<TY, TR, V, N, GATE>, a, s, blocks, false, st)
+void launch_forward(const NormArgs &a, const NormShape &s, bool wide, cudaStream_t st) {
+#define TMOE_RN(V, N) launch_walk<RowIn<TY, TR, V, N, GATE, false>>(residual_norm_kernel<TY, TR, V, N, GATE>, a, s, false, st)
   if (wide) { if (s.nv == 1) TMOE_RN(8, 1); else TMOE_RN(8, 2); }
   else { if (s.nv == 1) TMOE_RN(1, 8); else TMOE_RN(1, 16); }
 #undef TMOE_RN
 }
 
 template <typename TY, typename TR, bool GATE>
-void launch_backward(const NormArgs &a, const NormShape &s, bool wide, int blocks, cudaStream_t st) {
-#define TMOE_RNB(V, N) launch_walk<RowIn<TY, TR, V, N, GATE, true>>(residual_norm_backward_kernel<TY, TR, V, N, GATE>, a, s, blocks, true, st)
+void launch_backward(const NormArgs &a, const NormShape &s, bool wide, cudaStream_t st) {
+#define TMOE_RNB(V, N) launch_walk<RowIn<TY, TR, V, N, GATE, true>>(residual_norm_backward_kernel<TY, TR, V, N, GATE>, a, s, true, st)
   if (wide) { if (s.nv == 1) TMOE_RNB(8, 1); else TMOE_RNB(8, 2); }
   else { if (s.nv == 1) TMOE_RNB(1, 8); else TMOE_RNB(1, 16); }
 #undef TMOE_RNB
@@ -610,9 +686,9 @@ int tmoe_residual_norm(const tmoe_residual_norm_t *p, void *out, void *normed, f
   cudaStream_t st = (cudaStream_t)stream;
   const int sms = current_device_sms();
   if (sms <= 0) return TMOE_ERR_CUDA;
-  const NormShape s = norm_shape(p->d);
+  const NormShape s = norm_shape(p->rows, p->d, false, sms);
   a.tw = s.tw;
-  TMOE_NORM_TYPES(launch_forward, p, a, s, wide, norm_blocks(p->rows, p->d, false, sms), st);
+  TMOE_NORM_TYPES(launch_forward, p, a, s, wide, st);
   count_launch();
   return launch_status();
 }
@@ -621,7 +697,7 @@ int64_t tmoe_residual_norm_workspace_bytes(const tmoe_residual_norm_t *p) {
   int rc = check_norm(p);
   if (rc) return rc;
   // sized for up to 160 SMs, whatever device the sizing query runs on
-  return p->rows == 0 ? 0 : (int64_t)norm_blocks(p->rows, p->d, true, 160) * 2 * p->d * 4;
+  return p->rows == 0 ? 0 : (int64_t)norm_shape(p->rows, p->d, true, 160).blocks * 2 * p->d * 4;
 }
 
 int tmoe_residual_norm_backward(const tmoe_residual_norm_t *p, const float *rstd, const void *d_out, int64_t d_out_stride,
@@ -658,25 +734,24 @@ int tmoe_residual_norm_backward(const tmoe_residual_norm_t *p, const float *rstd
   if (d_next_w) a.sum_x = a.n_sums++;
   const int sms = current_device_sms();
   if (sms <= 0) return TMOE_ERR_CUDA;
-  const int blocks = norm_blocks(p->rows, p->d, true, sms < 160 ? sms : 160);
+  const NormShape s = norm_shape(p->rows, p->d, true, sms < 160 ? sms : 160);
   if (params) {
     if (!workspace) return TMOE_ERR_NULL;
-    if (workspace_bytes < (int64_t)blocks * a.n_sums * p->d * 4) return TMOE_ERR_WORKSPACE;
+    if (workspace_bytes < (int64_t)s.blocks * a.n_sums * p->d * 4) return TMOE_ERR_WORKSPACE;
     a.partial = reinterpret_cast<float *>(workspace);
   }
   const bool wide = norm_wide(*p) && wide_ok(d_out, d_out_stride, sr) && wide_ok(d_normed, d_normed_stride, sy) &&
                     wide_ok(d_y, p->d, sy) && wide_ok(d_residual, p->d, sr) && wide_ok(d_gate, p->d, sy);
-  const NormShape s = norm_shape(p->d);
   a.tw = s.tw;
-  TMOE_NORM_TYPES(launch_backward, p, a, s, wide, blocks, st);
+  TMOE_NORM_TYPES(launch_backward, p, a, s, wide, st);
   count_launch();
   if ((rc = launch_status())) return rc;
   if (params) {
     const int grid = (a.n_sums * p->d + 31) / 32;
     if (p->dtype == TMOE_F32)
-      norm_params_kernel<float><<<grid, 256, 0, st>>>(a, blocks, (float *)d_layer_scale, (float *)d_post_w, (float *)d_next_w);
+      norm_params_kernel<float><<<grid, 256, 0, st>>>(a, s.blocks, (float *)d_layer_scale, (float *)d_post_w, (float *)d_next_w);
     else
-      norm_params_kernel<bf16><<<grid, 256, 0, st>>>(a, blocks, (bf16 *)d_layer_scale, (bf16 *)d_post_w, (bf16 *)d_next_w);
+      norm_params_kernel<bf16><<<grid, 256, 0, st>>>(a, s.blocks, (bf16 *)d_layer_scale, (bf16 *)d_post_w, (bf16 *)d_next_w);
     count_launch();
     rc = launch_status();
   }
