@@ -30,11 +30,11 @@ namespace tmoe {
 namespace {
 
 constexpr int kMaxWidth = 8192;      // widest row: 512 threads x 16 elements
-// Warps of a block and blocks resident on an SM, by the registers a thread needs: forward 4 x 8 warps (64 registers) or larger blocks
-// of one row each; backward one block of 20 (96 registers).  Threads with 16 elements take 16 warps (128 registers).
-constexpr int kForwardWarps = 32, kBackwardWarps = 20, kWideWarps = 16;
-constexpr int resident_warps(int nv, bool back) { return nv == 2 ? kWideWarps : back ? kBackwardWarps : kForwardWarps; }
-constexpr int max_block(int nv, bool back) { return 32 * (nv == 2 ? kWideWarps : kBackwardWarps); }
+// Warps that an SM is meant to hold, by the registers a thread needs.  Forward 32 (64 registers) in blocks of 8 or of one row each;
+// backward one block of 20 (96 registers), or 16 (128) in fp32; 16 where a thread has 16 elements.
+constexpr int resident_warps(int nv, bool back, bool f32) { return nv == 2 ? 16 : back ? (f32 ? 16 : 20) : 32; }
+// Warps of the largest block: rows up to 8 columns a thread, beyond that 16 columns
+constexpr int block_warps(int nv, bool back, bool f32) { return back ? resident_warps(nv, back, f32) : 16; }
 constexpr int kRingBytes = 208 * 1024;
 
 // Two fp32 values worked on by one instruction: the walk is bound by the instructions it issues as much as by memory (80 a element in
@@ -64,6 +64,10 @@ __device__ __forceinline__ f2 sigmoid2(f2 g) {
 __device__ __forceinline__ void cp_async16(void *smem, const void *gmem) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ptx::smem_u32(smem)), "l"(gmem) : "memory");
 }
+// through L1: for two copies that share a 32-byte sector, so that it crosses from L2 once
+__device__ __forceinline__ void cp_async16_l1(void *smem, const void *gmem) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(ptx::smem_u32(smem)), "l"(gmem) : "memory");
+}
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
@@ -90,7 +94,7 @@ template <> struct Piece<bf16, 8> {
 template <> struct Piece<float, 8> {
   static constexpr int kPlanes = 2;
   float4 a, b;
-  __device__ static __forceinline__ void copy(uint4 *slot, int pitch, const float *p) { cp_async16(slot, p); cp_async16(slot + pitch, p + 4); }
+  __device__ static __forceinline__ void copy(uint4 *slot, int pitch, const float *p) { cp_async16_l1(slot, p); cp_async16_l1(slot + pitch, p + 4); }
   __device__ __forceinline__ void fetch(const uint4 *slot, int pitch) {
     a = *reinterpret_cast<const float4 *>(slot);
     b = *reinterpret_cast<const float4 *>(slot + pitch);
@@ -106,8 +110,7 @@ template <> struct Piece<float, 8> {
     return (j & 1) ? pair(v.z, v.w) : pair(v.x, v.y);
   }
   __device__ static __forceinline__ void store(float *p, const f2 *f) {
-    reinterpret_cast<ulonglong2 *>(p)[0] = make_ulonglong2(f[0], f[1]);
-    reinterpret_cast<ulonglong2 *>(p)[1] = make_ulonglong2(f[2], f[3]);
+    asm volatile("st.global.v4.b64 [%0], {%1, %2, %3, %4};" ::"l"(p), "l"(f[0]), "l"(f[1]), "l"(f[2]), "l"(f[3]) : "memory");
   }
 };
 template <typename T> struct Piece<T, 1> {
@@ -147,6 +150,8 @@ struct NormArgs {
   int64_t ys, rs, gs;                          // row strides in elements
   int64_t rows;
   int d, tw;                                   // row width; warps per row ("team")
+  int step;                                    // rows between two rows of one team: blocks * teams of a block
+  int64_t y_step, r_step, g_step, do_step, dn_step, o_step;   // step times the row strides, and times d
   float eps0, eps1;
   void *out, *normed;                          // forward outputs [rows, d]; either may be nullptr
   float *rstd;                                 // [2, rows]: 1/rms of y and of out; nullptr = not kept
@@ -169,22 +174,16 @@ template <int N> struct TeamRed {
   }
 };
 __device__ __forceinline__ float sum_places(const float (&v)[20], int tw) {
-  const float4 *p = reinterpret_cast<const float4 *>(v);
-  const float4 a = p[0];
-  float s = (a.x + a.y) + (a.z + a.w);
+  const ulonglong2 *p = reinterpret_cast<const ulonglong2 *>(v);
+  f2 s = add2(p[0].x, p[0].y);
   if (tw > 4) {
-    const float4 b = p[1];
-    s += (b.x + b.y) + (b.z + b.w);
+    s = add2(s, add2(p[1].x, p[1].y));
     if (tw > 8) {
-      const float4 c = p[2], d = p[3];
-      s += ((c.x + c.y) + (c.z + c.w)) + ((d.x + d.y) + (d.z + d.w));
-      if (tw > 16) {
-        const float4 e = p[4];
-        s += (e.x + e.y) + (e.z + e.w);
-      }
+      s = add2(s, add2(add2(p[2].x, p[2].y), add2(p[3].x, p[3].y)));
+      if (tw > 16) s = add2(s, add2(p[4].x, p[4].y));
     }
   }
-  return s;
+  return sum2(s);
 }
 __device__ __forceinline__ float team_sum(float v, int tw, int team, int slot, TeamRed<1> &red) {
   v = warp_sum(v);
@@ -225,7 +224,7 @@ template <typename TY, typename TR, int VEC, int NV, bool GATE, bool BACK> struc
   // as many rows ahead as fit for the warps that an SM is meant to run; below 2 stages rows are loaded when their turn comes
   // (backward, the parameters' columns of a thread lie behind the ring, in fp32)
   static constexpr int kParamPlanes = BACK && VEC == 8 ? 4 * NV : 0;
-  static constexpr int kFit = kPlanes ? (kRingBytes / (resident_warps(NV, BACK) * 512) - kParamPlanes) / kPlanes : 0;
+  static constexpr int kFit = kPlanes ? (kRingBytes / (resident_warps(NV, BACK, sizeof(TY) == 4) * 512) - kParamPlanes) / kPlanes : 0;
   static constexpr int kStages = kFit >= 3 ? 3 : kFit == 2 ? 2 : 1;
   static constexpr bool kRing = kStages > 1;
   PY y[NV], g[GATE ? NV : 1], dn[BACK ? NV : 1];
@@ -239,34 +238,34 @@ template <typename TY, typename TR, int VEC, int NV, bool GATE, bool BACK> struc
   // this thread's first piece in the row that is copied (or, without a ring, loaded) next
   const TY *y, *g, *dn;
   const TR *r, *o;
-  int64_t ahead;       // that row
+  int ahead;           // that row (rows + 3 * step < 2^31)
   uint4 *slot;
   int stage;
 
-  __device__ __forceinline__ RowWalk(const NormArgs &a, int64_t row, int64_t step, int lt) : ahead(row), slot(norm_ring + threadIdx.x), stage(0) {
-    y = (const TY *)a.y + row * a.ys + lt * VEC;
-    g = (const TY *)a.gate + row * a.gs + lt * VEC;
-    dn = (const TY *)a.d_normed + row * a.dns + lt * VEC;
-    r = (const TR *)a.res + row * a.rs + lt * VEC;
-    o = (const TR *)a.d_out + row * a.dos + lt * VEC;
+  __device__ __forceinline__ RowWalk(const NormArgs &a, int row, int lt) : ahead(row), slot(norm_ring + threadIdx.x), stage(0) {
+    y = (const TY *)a.y + (int64_t)row * a.ys + lt * VEC;
+    g = (const TY *)a.gate + (int64_t)row * a.gs + lt * VEC;
+    dn = (const TY *)a.d_normed + (int64_t)row * a.dns + lt * VEC;
+    r = (const TR *)a.res + (int64_t)row * a.rs + lt * VEC;
+    o = (const TR *)a.d_out + (int64_t)row * a.dos + lt * VEC;
     if (In::kRing) {
 #pragma unroll
       for (int i = 0; i < In::kStages * In::kPlanes; ++i) slot[i * blockDim.x] = make_uint4(0, 0, 0, 0);
 #pragma unroll
-      for (int s = 0; s < In::kStages - 1; ++s) copy(a, step, lt, at(s));
+      for (int s = 0; s < In::kStages - 1; ++s) copy(a, lt, at(s));
     }
   }
   __device__ __forceinline__ uint4 *at(int s) const { return slot + s * In::kPlanes * blockDim.x; }
   __device__ __forceinline__ uint4 *behind() const { return at(In::kStages); }
-  __device__ __forceinline__ void advance(const NormArgs &a, int64_t step) {
-    ahead += step;
-    y += step * a.ys;
-    r += step * a.rs;
-    if (GATE) g += step * a.gs;
-    if (BACK) { dn += step * a.dns; o += step * a.dos; }
+  __device__ __forceinline__ void advance(const NormArgs &a) {
+    ahead += a.step;
+    y += a.y_step;
+    r += a.r_step;
+    if (GATE) g += a.g_step;
+    if (BACK) { dn += a.dn_step; o += a.do_step; }
   }
-  __device__ __forceinline__ void copy(const NormArgs &a, int64_t step, int lt, uint4 *to) {
-    if (ahead < a.rows) {
+  __device__ __forceinline__ void copy(const NormArgs &a, int lt, uint4 *to) {
+    if (ahead < (int)a.rows) {
       const int pitch = blockDim.x, tpr = a.tw * 32;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
@@ -281,7 +280,7 @@ template <typename TY, typename TR, int VEC, int NV, bool GATE, bool BACK> struc
         to += In::kPlanes / NV * pitch;
       }
     }
-    advance(a, step);
+    advance(a);
     cp_async_commit();
   }
   // planes of one piece: y, gate, residual, d_normed, d_out
@@ -297,9 +296,9 @@ template <typename TY, typename TR, int VEC, int NV, bool GATE, bool BACK> struc
       from += In::kPlanes / NV * pitch;
     }
   }
-  __device__ __forceinline__ void take(const NormArgs &a, int64_t step, int lt, In &in) {
+  __device__ __forceinline__ void take(const NormArgs &a, int lt, In &in) {
     if (In::kRing) {
-      copy(a, step, lt, at(stage == 0 ? In::kStages - 1 : stage - 1));
+      copy(a, lt, at(stage == 0 ? In::kStages - 1 : stage - 1));
       cp_async_wait<In::kStages - 1>();
       fetch(at(stage), in);
       stage = stage + 1 == In::kStages ? 0 : stage + 1;
@@ -321,7 +320,7 @@ template <typename TY, typename TR, int VEC, int NV, bool GATE, bool BACK> struc
           }
         }
       }
-      advance(a, step);
+      advance(a);
     }
   }
   // the row taken last, once more
@@ -367,21 +366,21 @@ template <typename TY, int VEC, int NV> struct Params {
 
 // A team walks over rows blockIdx * teams + team, + gridDim * teams, ...
 template <typename TY, typename TR, int VEC, int NV, bool GATE>
-__global__ void __launch_bounds__(VEC == 8 && NV == 1 ? 512 : max_block(VEC == 8 ? NV : NV / 8, false), VEC == 8 && NV == 1 ? 2 : 1) residual_norm_kernel(const __grid_constant__ NormArgs a) {
+__global__ void __launch_bounds__(512, VEC == 8 && NV == 1 ? 2 : 1) residual_norm_kernel(const __grid_constant__ NormArgs a) {
   using In = RowIn<TY, TR, VEC, NV, GATE, false>;
   __shared__ __align__(16) TeamRed<1> red;
   red.init();
   const int tpr = a.tw * 32, team = threadIdx.x / tpr, lt = threadIdx.x - team * tpr;
-  const int64_t step = (int64_t)gridDim.x * (blockDim.x / tpr);
-  int64_t row = (int64_t)blockIdx.x * (blockDim.x / tpr) + team;
+  int row = blockIdx.x * (blockDim.x / tpr) + team;
+  int64_t off = (int64_t)row * a.d;     // of the row in the outputs
   const float inv_d = 1.f / (float)a.d;
-  RowWalk<TY, TR, VEC, NV, GATE, false> walk(a, row, step, lt);
+  RowWalk<TY, TR, VEC, NV, GATE, false> walk(a, row, lt);
   Params<TY, VEC, NV> w;
   w.load(a, lt);
   int slot = 0;
-  for (; row < a.rows; row += step) {
+  for (; row < (int)a.rows; row += a.step, off += a.o_step) {
     In in;
-    walk.take(a, step, lt, in);
+    walk.take(a, lt, in);
     constexpr int N2 = NV * VEC / 2;
     float rho0 = 1.f;
     if (a.w0) {
@@ -400,14 +399,14 @@ __global__ void __launch_bounds__(VEC == 8 && NV == 1 ? 512 : max_block(VEC == 8
       v[j] = add2(t, pair_of(in.r, j));
       ss = fma2(v[j], v[j], ss);
     }
-    if (a.out) store_row<TR, VEC, NV>((TR *)a.out + row * a.d, tpr, lt, a.d, v);
+    if (a.out) store_row<TR, VEC, NV>((TR *)a.out + off, tpr, lt, a.d, v);
     if (!a.normed) continue;
     const float rho1 = rsqrtf(fmaf(team_sum(sum2(ss), a.tw, team, slot, red), inv_d, a.eps1));
     slot ^= 1;
     if (a.rstd && lt == 0) a.rstd[a.rows + row] = rho1;
 #pragma unroll
     for (int j = 0; j < N2; ++j) v[j] = mul2(v[j], mul2(both(rho1), w.w1[j]));
-    store_row<TY, VEC, NV>((TY *)a.normed + row * a.d, tpr, lt, a.d, v);
+    store_row<TY, VEC, NV>((TY *)a.normed + off, tpr, lt, a.d, v);
   }
 }
 
@@ -416,15 +415,15 @@ __global__ void __launch_bounds__(VEC == 8 && NV == 1 ? 512 : max_block(VEC == 8
 // adds its teams in order and writes one row of partial sums; norm_params_kernel adds the blocks in order.  The result depends on the
 // sizes and the grid only.
 template <typename TY, typename TR, int VEC, int NV, bool GATE>
-__global__ void __launch_bounds__(max_block(VEC == 8 ? NV : NV / 8, true)) residual_norm_backward_kernel(const __grid_constant__ NormArgs a) {
+__global__ void __launch_bounds__(32 * block_warps(VEC == 8 ? NV : NV / 8, true, sizeof(TY) == 4)) residual_norm_backward_kernel(const __grid_constant__ NormArgs a) {
   using In = RowIn<TY, TR, VEC, NV, GATE, true>;
   __shared__ __align__(16) TeamRed<3> red;
   red.init();
   const int tpr = a.tw * 32, team = threadIdx.x / tpr, lt = threadIdx.x - team * tpr, teams = blockDim.x / tpr;
-  const int64_t step = (int64_t)gridDim.x * teams;
-  int64_t row = (int64_t)blockIdx.x * teams + team;
+  int row = blockIdx.x * teams + team;
+  int64_t off = (int64_t)row * a.d;     // of the row in the outputs
   const float inv_d = 1.f / (float)a.d;
-  RowWalk<TY, TR, VEC, NV, GATE, true> walk(a, row, step, lt);
+  RowWalk<TY, TR, VEC, NV, GATE, true> walk(a, row, lt);
   // Registers are what decides how many rows an SM works on.  With a ring a thread reads its pieces of the row and of the parameters
   // from shared memory in both passes over the row, so that only x, b and the sums stay in registers across the reduction.
   Params<TY, VEC, NV> w;
@@ -436,15 +435,18 @@ __global__ void __launch_bounds__(max_block(VEC == 8 ? NV : NV / 8, true)) resid
   for (int j = 0; j < N2; ++j) acc_a[j] = acc_x[j] = both(0.f);
   int slot = 0;
   // without dN nothing flows through the next norm; one row's rstd are loaded a row ahead
-  float next0 = a.w0 && row < a.rows ? a.rstd[row] : 1.f, next1 = a.d_normed && row < a.rows ? a.rstd[a.rows + row] : 0.f;
-  for (; row < a.rows; row += step) {
+  const float *rstd0 = a.rstd + row, *rstd1 = rstd0 + a.rows;
+  float next0 = a.w0 && row < (int)a.rows ? *rstd0 : 1.f, next1 = a.d_normed && row < (int)a.rows ? *rstd1 : 0.f;
+  for (; row < (int)a.rows; row += a.step, off += a.o_step) {
     const float rho0 = next0, rho1 = next1;
-    if (row + step < a.rows) {
-      if (a.w0) next0 = a.rstd[row + step];
-      if (a.d_normed) next1 = a.rstd[a.rows + row + step];
+    rstd0 += a.step;
+    rstd1 += a.step;
+    if (row + a.step < (int)a.rows) {
+      if (a.w0) next0 = *rstd0;
+      if (a.d_normed) next1 = *rstd1;
     }
     In in;
-    walk.take(a, step, lt, in);
+    walk.take(a, lt, in);
     if (In::kRing) w.fetch(walk.behind());
     f2 x[N2], b[N2], s1 = both(0.f), s2 = s1, s3 = s1;   // sum u*x, sum q*b, sum q*x
     const f2 r0 = both(rho0), r1 = both(rho1);
@@ -476,7 +478,7 @@ __global__ void __launch_bounds__(max_block(VEC == 8 ? NV : NV / 8, true)) resid
       b[j] = fma2(n1, x[j], b[j]);                                     // dR
       acc_x[j] = fma2(pair_of(in.dn, j), x[j], acc_x[j]);
     }
-    if (a.d_res) store_row<TR, VEC, NV>((TR *)a.d_res + row * a.d, tpr, lt, a.d, b);
+    if (a.d_res) store_row<TR, VEC, NV>((TR *)a.d_res + off, tpr, lt, a.d, b);
     if (GATE) {
       f2 f[N2];
 #pragma unroll
@@ -487,7 +489,7 @@ __global__ void __launch_bounds__(max_block(VEC == 8 ? NV : NV / 8, true)) resid
         f[j] = mul2(mul2(b[j], ch), fma2(s, fma2(sg, both(-1.f), both(1.f)), sg));
         b[j] = mul2(b[j], s);                                          // dR * s
       }
-      if (a.d_gate) store_row<TY, VEC, NV>((TY *)a.d_gate + row * a.d, tpr, lt, a.d, f);
+      if (a.d_gate) store_row<TY, VEC, NV>((TY *)a.d_gate + off, tpr, lt, a.d, f);
     }
 #pragma unroll
     for (int j = 0; j < N2; ++j) {
@@ -495,7 +497,7 @@ __global__ void __launch_bounds__(max_block(VEC == 8 ? NV : NV / 8, true)) resid
       acc_a[j] = fma2(b[j], h, acc_a[j]);
       b[j] = fma2(mul2(b[j], r0), w.c[j], mul2(n0, h));
     }
-    if (a.d_y) store_row<TY, VEC, NV>((TY *)a.d_y + row * a.d, tpr, lt, a.d, b);
+    if (a.d_y) store_row<TY, VEC, NV>((TY *)a.d_y + off, tpr, lt, a.d, b);
   }
   if (!a.partial) return;
   // [d] floats where the ring was, when a block has several teams: all of its copies have landed and been read by then
@@ -561,12 +563,12 @@ struct NormShape { int tw, nv, teams, blocks; };
 // Warps per row, pieces per thread, rows worked on at once by a block, blocks.  One 8-element piece per thread where a row's warps then
 // fit a block: a row spread over several warps costs a barrier, but leaves registers and shared memory for the rows ahead.  Few rows are
 // spread over the SMs before a block takes several.
-NormShape norm_shape(int64_t rows, int d, bool back, int sms) {
+NormShape norm_shape(int64_t rows, int d, bool back, bool f32, int sms) {
   NormShape s;
   const int pieces = (d + 7) / 8;
-  s.nv = pieces <= 32 * (back ? kBackwardWarps : kWideWarps) ? 1 : 2;
+  s.nv = pieces <= 32 * block_warps(1, back, f32) ? 1 : 2;
   s.tw = (pieces + 32 * s.nv - 1) / (32 * s.nv);
-  const int resident = resident_warps(s.nv, back), full = back ? resident : 8;
+  const int resident = resident_warps(s.nv, back, f32), full = back ? resident : 8;
   s.teams = s.tw >= full ? 1 : full / s.tw;
   if (s.tw > 1 && s.teams > 10) s.teams = 10;
   const int64_t each = (rows + sms - 1) / sms;
@@ -577,9 +579,8 @@ NormShape norm_shape(int64_t rows, int d, bool back, int sms) {
 }
 
 bool bad_align(const void *p, int size) { return p && (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(size - 1)); }
-bool wide_ok(const void *p, int64_t stride, int size) {
-  return !p || (!(reinterpret_cast<uintptr_t>(p) & 15) && (stride * size) % 16 == 0);
-}
+// rows of 8-element pieces that each start on a multiple of their size (16 bytes in bf16, 32 in fp32)
+bool wide_ok(const void *p, int64_t stride, int size) { return !p || (!(reinterpret_cast<uintptr_t>(p) & (8 * size - 1)) && stride % 8 == 0); }
 
 int check_norm(const tmoe_residual_norm_t *p) {
   if (!p) return TMOE_ERR_NULL;
@@ -607,7 +608,7 @@ NormArgs norm_args(const tmoe_residual_norm_t &p) {
   return a;
 }
 
-// 16-byte pieces when every row of every tensor starts on a 16-byte boundary and the width is a multiple of 8
+// 8-element pieces when every row of every tensor starts on a piece's boundary and the width is a multiple of 8
 bool norm_wide(const tmoe_residual_norm_t &p) {
   const int sy = p.dtype == TMOE_F32 ? 4 : 2, sr = p.residual_dtype == TMOE_F32 ? 4 : 2;
   return p.d % 8 == 0 && wide_ok(p.y, p.y_stride, sy) && wide_ok(p.gate, p.gate_stride, sy) &&
@@ -631,7 +632,11 @@ void launch_walk(Kernel kernel, const NormArgs &a, const NormShape &s, bool fold
     cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     opted.fetch_or(bit, std::memory_order_relaxed);
   }
-  kernel<<<s.blocks, threads, smem, st>>>(a);
+  NormArgs b = a;
+  b.step = s.blocks * s.teams;
+  b.y_step = b.step * a.ys; b.r_step = b.step * a.rs; b.g_step = b.step * a.gs; b.do_step = b.step * a.dos; b.dn_step = b.step * a.dns;
+  b.o_step = (int64_t)b.step * a.d;
+  kernel<<<s.blocks, threads, smem, st>>>(b);
 }
 
 template <typename TY, typename TR, bool GATE>
@@ -686,7 +691,7 @@ int tmoe_residual_norm(const tmoe_residual_norm_t *p, void *out, void *normed, f
   cudaStream_t st = (cudaStream_t)stream;
   const int sms = current_device_sms();
   if (sms <= 0) return TMOE_ERR_CUDA;
-  const NormShape s = norm_shape(p->rows, p->d, false, sms);
+  const NormShape s = norm_shape(p->rows, p->d, false, p->dtype == TMOE_F32, sms);
   a.tw = s.tw;
   TMOE_NORM_TYPES(launch_forward, p, a, s, wide, st);
   count_launch();
@@ -697,7 +702,7 @@ int64_t tmoe_residual_norm_workspace_bytes(const tmoe_residual_norm_t *p) {
   int rc = check_norm(p);
   if (rc) return rc;
   // sized for up to 160 SMs, whatever device the sizing query runs on
-  return p->rows == 0 ? 0 : (int64_t)norm_shape(p->rows, p->d, true, 160).blocks * 2 * p->d * 4;
+  return p->rows == 0 ? 0 : (int64_t)norm_shape(p->rows, p->d, true, p->dtype == TMOE_F32, 160).blocks * 2 * p->d * 4;
 }
 
 int tmoe_residual_norm_backward(const tmoe_residual_norm_t *p, const float *rstd, const void *d_out, int64_t d_out_stride,
@@ -734,7 +739,7 @@ int tmoe_residual_norm_backward(const tmoe_residual_norm_t *p, const float *rstd
   if (d_next_w) a.sum_x = a.n_sums++;
   const int sms = current_device_sms();
   if (sms <= 0) return TMOE_ERR_CUDA;
-  const NormShape s = norm_shape(p->rows, p->d, true, sms < 160 ? sms : 160);
+  const NormShape s = norm_shape(p->rows, p->d, true, p->dtype == TMOE_F32, sms < 160 ? sms : 160);
   if (params) {
     if (!workspace) return TMOE_ERR_NULL;
     if (workspace_bytes < (int64_t)s.blocks * a.n_sums * p->d * 4) return TMOE_ERR_WORKSPACE;
