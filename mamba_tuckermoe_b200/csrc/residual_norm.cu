@@ -33,8 +33,9 @@ constexpr int kMaxWidth = 8192;      // widest row: 512 threads x 16 elements
 // Warps that an SM is meant to hold, by the registers a thread needs.  Forward 32 (64 registers) in blocks of 8 or of one row each;
 // backward one block of 20 (96 registers), or 16 (128) in fp32; 16 where a thread has 16 elements.
 constexpr int resident_warps(int nv, bool back, bool f32) { return nv == 2 ? 16 : back ? (f32 ? 16 : 20) : 32; }
-// Warps of the largest block: rows up to 8 columns a thread, beyond that 16 columns
+// Warps of the largest block
 constexpr int block_warps(int nv, bool back, bool f32) { return back ? resident_warps(nv, back, f32) : 16; }
+constexpr int kMaxTeams = 10;           // teams of several warps in a block (a named barrier each)
 constexpr int kRingBytes = 208 * 1024;
 
 // Two fp32 values worked on by one instruction: the walk is bound by the instructions it issues as much as by memory (80 a element in
@@ -167,9 +168,9 @@ struct NormArgs {
 // Sums over the `tw` warps of a team, in a fixed order.  A team has 20 places of shared memory for each sum, zero beyond its own warps
 // (TeamRed::init), which every thread reads back with wide loads; `slot` alternates between calls, so one barrier per call is enough.
 template <int N> struct TeamRed {
-  float at[2][10][N][20];   // [slot][team][sum][warp]
+  float at[2][kMaxTeams][N][20];   // [slot][team][sum][warp]
   __device__ __forceinline__ void init() {
-    for (int i = threadIdx.x; i < 2 * 10 * N * 20; i += blockDim.x) (&at[0][0][0][0])[i] = 0.f;
+    for (int i = threadIdx.x; i < 2 * kMaxTeams * N * 20; i += blockDim.x) (&at[0][0][0][0])[i] = 0.f;
     __syncthreads();
   }
 };
@@ -560,23 +561,34 @@ __global__ void __launch_bounds__(256) norm_params_kernel(const __grid_constant_
 
 struct NormShape { int tw, nv, teams, blocks; };
 
-// Warps per row, pieces per thread, rows worked on at once by a block, blocks.  One 8-element piece per thread where a row's warps then
-// fit a block: a row spread over several warps costs a barrier, but leaves registers and shared memory for the rows ahead.  Few rows are
-// spread over the SMs before a block takes several.
-NormShape norm_shape(int64_t rows, int d, bool back, bool f32, int sms) {
+// Warps per row, 8-element pieces per thread, rows worked on at once by a block, blocks.
+//
+// Two pieces a thread halve what a row costs besides its elements (reduction, barrier, addresses); one piece leaves room for more
+// threads and, on few rows, is quicker through its chain.  Measured over 37.7 M elements with all operands but the gate, one / two:
+// forward d = 384: 52.9 / 55.4 us, 768: 64.0 / 50.8, 2304: 54.4 / 49.6, 4096: 53.9 / 49.5; backward d = 768: 85.3 / 88.4, 1536:
+// 93.8 / 82.1, 2304: 107.8 / 87.9, 4096: 112.2 / 88.1.  Backward with a gate, or in fp32, two pieces' ring does not fit (or their registers
+// spill): 310 us against 78 us at 768 with a gate.  Few rows are spread over the SMs before a block takes several.
+NormShape norm_shape(const tmoe_residual_norm_t &p, bool back, int sms) {
   NormShape s;
-  const int pieces = (d + 7) / 8;
-  s.nv = pieces <= 32 * block_warps(1, back, f32) ? 1 : 2;
+  const bool f32 = p.dtype == TMOE_F32;
+  const int64_t rows = p.rows;
+  const int pieces = (p.d + 7) / 8;
+  const bool two = back ? pieces > 128 && !f32 && p.residual_dtype == TMOE_BF16 && !p.gate : pieces > 64;
+  s.nv = pieces > 32 * block_warps(1, back, f32) || (two && rows > sms) ? 2 : 1;
   s.tw = (pieces + 32 * s.nv - 1) / (32 * s.nv);
   const int resident = resident_warps(s.nv, back, f32), full = back ? resident : 8;
   s.teams = s.tw >= full ? 1 : full / s.tw;
-  if (s.tw > 1 && s.teams > 10) s.teams = 10;
+  if (s.tw > 1 && s.teams > kMaxTeams) s.teams = kMaxTeams;
   const int64_t each = (rows + sms - 1) / sms;
   if (each < s.teams) s.teams = each < 1 ? 1 : (int)each;
-  const int64_t want = (rows + s.teams - 1) / s.teams, cap = (int64_t)sms * (back ? 1 : resident / (s.tw * s.teams) > 0 ? resident / (s.tw * s.teams) : 1);
+  const int per_sm = back || s.tw * s.teams > resident ? 1 : resident / (s.tw * s.teams);
+  const int64_t want = (rows + s.teams - 1) / s.teams, cap = (int64_t)sms * per_sm;
   s.blocks = (int)(want < cap ? want : cap);
   return s;
 }
+
+// Blocks of the backward walk at most: one on each SM (sized for up to 160, whatever device a sizing query runs on)
+int64_t max_partials(int64_t rows) { return rows < 160 ? rows : 160; }
 
 bool bad_align(const void *p, int size) { return p && (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(size - 1)); }
 // rows of 8-element pieces that each start on a multiple of their size (16 bytes in bf16, 32 in fp32)
@@ -691,7 +703,7 @@ int tmoe_residual_norm(const tmoe_residual_norm_t *p, void *out, void *normed, f
   cudaStream_t st = (cudaStream_t)stream;
   const int sms = current_device_sms();
   if (sms <= 0) return TMOE_ERR_CUDA;
-  const NormShape s = norm_shape(p->rows, p->d, false, p->dtype == TMOE_F32, sms);
+  const NormShape s = norm_shape(*p, false, sms);
   a.tw = s.tw;
   TMOE_NORM_TYPES(launch_forward, p, a, s, wide, st);
   count_launch();
@@ -701,8 +713,7 @@ int tmoe_residual_norm(const tmoe_residual_norm_t *p, void *out, void *normed, f
 int64_t tmoe_residual_norm_workspace_bytes(const tmoe_residual_norm_t *p) {
   int rc = check_norm(p);
   if (rc) return rc;
-  // sized for up to 160 SMs, whatever device the sizing query runs on
-  return p->rows == 0 ? 0 : (int64_t)norm_shape(p->rows, p->d, true, p->dtype == TMOE_F32, 160).blocks * 2 * p->d * 4;
+  return p->rows == 0 ? 0 : max_partials(p->rows) * 2 * p->d * 4;
 }
 
 int tmoe_residual_norm_backward(const tmoe_residual_norm_t *p, const float *rstd, const void *d_out, int64_t d_out_stride,
@@ -739,10 +750,10 @@ int tmoe_residual_norm_backward(const tmoe_residual_norm_t *p, const float *rstd
   if (d_next_w) a.sum_x = a.n_sums++;
   const int sms = current_device_sms();
   if (sms <= 0) return TMOE_ERR_CUDA;
-  const NormShape s = norm_shape(p->rows, p->d, true, p->dtype == TMOE_F32, sms < 160 ? sms : 160);
+  const NormShape s = norm_shape(*p, true, sms < 160 ? sms : 160);
   if (params) {
     if (!workspace) return TMOE_ERR_NULL;
-    if (workspace_bytes < (int64_t)s.blocks * a.n_sums * p->d * 4) return TMOE_ERR_WORKSPACE;
+    if (workspace_bytes < max_partials(p->rows) * a.n_sums * p->d * 4) return TMOE_ERR_WORKSPACE;
     a.partial = reinterpret_cast<float *>(workspace);
   }
   const bool wide = norm_wide(*p) && wide_ok(d_out, d_out_stride, sr) && wide_ok(d_normed, d_normed_stride, sy) &&
