@@ -265,14 +265,15 @@ typedef struct tmoe_route {
   const uint8_t *token_mask; /* [tokens], or NULL: every token counts */
 } tmoe_route_t;
 int64_t tmoe_route_workspace_bytes(const tmoe_route_t *p);   /* of the forward call */
-/* idx, gates [tokens, top_k] (descending score), counts [n_experts], losses [3] */
-int tmoe_route_tokens(const tmoe_route_t *p, int32_t *idx, float *gates, int32_t *counts, float *losses, void *workspace,
+/* idx, gates [tokens, top_k] (descending score), counts [n_experts], losses [3]; stats [tokens, 2], 8-byte
+ * aligned: what the backward call needs of the tokens that count (largest logit, sum of exp(logit - largest)), or NULL */
+int tmoe_route_tokens(const tmoe_route_t *p, int32_t *idx, float *gates, int32_t *counts, float *losses, float *stats, void *workspace,
                       int64_t workspace_bytes, void *stream);
 /* d_scores [tokens, n_experts] (dtype) from the forward call's results and the upstream gradients d_gates [tokens, top_k],
  * d_balance and d_z (one float each, on the device); each may be NULL (zero).  counts carry no gradient. */
 int tmoe_route_tokens_backward(const tmoe_route_t *p, const int32_t *idx, const float *gates, const int32_t *counts,
-                               const float *losses, const float *d_gates, const float *d_balance, const float *d_z, void *d_scores,
-                               void *stream);
+                               const float *losses, const float *stats, const float *d_gates, const float *d_balance,
+                               const float *d_z, void *d_scores, void *stream);
 
 /* c[t] = sum_j gates[t, j] * U_expert[idx[t, j]] (pure_torch_mlx/model.py:93 folded through the core mixing): the coefficients
  * that tmoe_in_core takes.  A slot whose index lies outside 0 .. n_experts-1 is empty. */

@@ -135,9 +135,9 @@ def load():
         lib.tmoe_route_workspace_bytes.restype = i64
         lib.tmoe_route_workspace_bytes.argtypes = [RP]
         lib.tmoe_route_tokens.restype = i32
-        lib.tmoe_route_tokens.argtypes = [RP, vp, vp, vp, vp, vp, i64, vp]
+        lib.tmoe_route_tokens.argtypes = [RP, vp, vp, vp, vp, vp, vp, i64, vp]
         lib.tmoe_route_tokens_backward.restype = i32
-        lib.tmoe_route_tokens_backward.argtypes = [RP] + [vp] * 9
+        lib.tmoe_route_tokens_backward.argtypes = [RP] + [vp] * 10
         lib.tmoe_expert_coef.restype = i32
         lib.tmoe_expert_coef.argtypes = [XP, vp, vp]
         lib.tmoe_expert_coef_workspace_bytes.restype = i64

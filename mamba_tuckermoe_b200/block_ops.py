@@ -269,7 +269,8 @@ def _route_struct(s2, mask, top_k, router) -> Route:
                  _ptr(mask))
 
 
-def _route_forward(scores, mask, top_k, router):
+def _route_forward(scores, mask, top_k, router, keep=False):
+    """(idx, gates, counts, losses, stats or None)"""
     _check_route(scores, top_k, mask)
     E, lead, dev = scores.shape[-1], scores.shape[:-1], scores.device
     s2 = _rows(scores, E)
@@ -279,19 +280,20 @@ def _route_forward(scores, mask, top_k, router):
     gates = torch.empty((*lead, top_k), dtype=torch.float32, device=dev)
     counts = torch.empty(E, dtype=torch.int32, device=dev)
     losses = torch.empty(3, dtype=torch.float32, device=dev)
+    stats = torch.empty((*lead, 2), dtype=torch.float32, device=dev) if keep else None
     p = _route_struct(s2, mask, top_k, router)
     lib = _lib.load()
     with _on(dev) as stream:
         n = _lib.check(lib.tmoe_route_workspace_bytes(C.byref(p)), "tmoe_route_workspace_bytes")
         ws = torch.empty(n, dtype=torch.uint8, device=dev)
-        rc = lib.tmoe_route_tokens(C.byref(p), idx.data_ptr(), gates.data_ptr(), counts.data_ptr(), losses.data_ptr(), ws.data_ptr(),
-                                   n, stream)
+        rc = lib.tmoe_route_tokens(C.byref(p), idx.data_ptr(), gates.data_ptr(), counts.data_ptr(), losses.data_ptr(), _ptr(stats),
+                                   ws.data_ptr(), n, stream)
     if rc < 0:
         _lib.check(rc, "tmoe_route_tokens")
-    return idx, gates, counts, losses
+    return idx, gates, counts, losses, stats
 
 
-def _route_backward(scores, mask, idx, gates, counts, losses, top_k, router, d_gates, d_balance, d_z):
+def _route_backward(scores, mask, idx, gates, counts, losses, stats, top_k, router, d_gates, d_balance, d_z):
     E = scores.shape[-1]
     s2 = _rows(scores, E)
     if mask is not None and not mask.is_contiguous():
@@ -301,7 +303,7 @@ def _route_backward(scores, mask, idx, gates, counts, losses, top_k, router, d_g
     p = _route_struct(s2, mask, top_k, router)
     with _on(scores.device) as stream:
         rc = _lib.load().tmoe_route_tokens_backward(C.byref(p), idx.data_ptr(), gates.data_ptr(), counts.data_ptr(), losses.data_ptr(),
-                                                    _ptr(d_gates), _ptr(d_balance), _ptr(d_z), d_scores.data_ptr(), stream)
+                                                    stats.data_ptr(), _ptr(d_gates), _ptr(d_balance), _ptr(d_z), d_scores.data_ptr(), stream)
     if rc < 0:
         _lib.check(rc, "tmoe_route_tokens_backward")
     return d_scores
@@ -311,9 +313,9 @@ class _RouteTokens(torch.autograd.Function):
     @staticmethod
     def forward(ctx, scores, mask, top_k, router):
         ctx.set_materialize_grads(False)
-        idx, gates, counts, losses = _route_forward(scores, mask, top_k, router)
+        idx, gates, counts, losses, stats = _route_forward(scores, mask, top_k, router, True)
         ctx.mark_non_differentiable(idx, counts)
-        ctx.save_for_backward(scores, mask, idx, gates, counts, losses)
+        ctx.save_for_backward(scores, mask, idx, gates, counts, losses, stats)
         ctx.top_k, ctx.router = top_k, router
         return idx, gates, counts, losses[0].clone(), losses[1].clone()
 
@@ -327,28 +329,29 @@ class _RouteTokens(torch.autograd.Function):
 
 @torch.library.custom_op("tmoe_b200::route_tokens", mutates_args=())
 def _route_tokens_op(scores: torch.Tensor, mask: Optional[torch.Tensor], top_k: int, router_mode: int, router_cap: float,
-                     router_temperature: float) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-    """(idx, gates, counts, losses); losses = balance, z and the number of tokens that count."""
-    return _route_forward(scores, mask, top_k, (router_mode, router_cap, router_temperature))
+                     router_temperature: float) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(idx, gates, counts, losses, stats); losses = balance, z and the number of tokens that count."""
+    return _route_forward(scores, mask, top_k, (router_mode, router_cap, router_temperature), True)
 
 
 @_route_tokens_op.register_fake
 def _(scores, mask, top_k, router_mode, router_cap, router_temperature):
     return (scores.new_empty((*scores.shape[:-1], top_k), dtype=torch.int32),
             scores.new_empty((*scores.shape[:-1], top_k), dtype=torch.float32),
-            scores.new_empty((scores.shape[-1],), dtype=torch.int32), scores.new_empty((3,), dtype=torch.float32))
+            scores.new_empty((scores.shape[-1],), dtype=torch.int32), scores.new_empty((3,), dtype=torch.float32),
+            scores.new_empty((*scores.shape[:-1], 2), dtype=torch.float32))
 
 
 @torch.library.custom_op("tmoe_b200::route_tokens_backward", mutates_args=())
 def _route_tokens_backward_op(scores: torch.Tensor, mask: Optional[torch.Tensor], idx: torch.Tensor, gates: torch.Tensor,
-                              counts: torch.Tensor, losses: torch.Tensor, top_k: int, router_mode: int, router_cap: float,
+                              counts: torch.Tensor, losses: torch.Tensor, stats: torch.Tensor, top_k: int, router_mode: int, router_cap: float,
                               router_temperature: float, d_gates: torch.Tensor, d_losses: torch.Tensor) -> torch.Tensor:
-    return _route_backward(scores, mask, idx, gates, counts, losses, top_k, (router_mode, router_cap, router_temperature), d_gates,
+    return _route_backward(scores, mask, idx, gates, counts, losses, stats, top_k, (router_mode, router_cap, router_temperature), d_gates,
                            d_losses[0], d_losses[1])
 
 
 @_route_tokens_backward_op.register_fake
-def _(scores, mask, idx, gates, counts, losses, top_k, router_mode, router_cap, router_temperature, d_gates, d_losses):
+def _(scores, mask, idx, gates, counts, losses, stats, top_k, router_mode, router_cap, router_temperature, d_gates, d_losses):
     return scores.new_empty(scores.shape)
 
 
@@ -356,12 +359,12 @@ def _route_op_setup(ctx, inputs, output):
     scores, mask, *rule = inputs
     ctx.rule, ctx.has_mask = rule, mask is not None
     ctx.save_for_backward(scores, *output, *([mask] if mask is not None else []))
-    ctx.mark_non_differentiable(output[0], output[2])
+    ctx.mark_non_differentiable(output[0], output[2], output[4])
 
 
-def _route_op_backward(ctx, d_idx, d_gates, d_counts, d_losses):
-    scores, idx, gates, counts, losses, *mask = ctx.saved_tensors
-    d = torch.ops.tmoe_b200.route_tokens_backward(scores, mask[0] if mask else None, idx, gates, counts, losses, *ctx.rule, d_gates, d_losses)
+def _route_op_backward(ctx, d_idx, d_gates, d_counts, d_losses, d_stats):
+    scores, idx, gates, counts, losses, stats, *mask = ctx.saved_tensors
+    d = torch.ops.tmoe_b200.route_tokens_backward(scores, mask[0] if mask else None, idx, gates, counts, losses, stats, *ctx.rule, d_gates, d_losses)
     return (d, None, None, None, None, None)
 
 
@@ -384,11 +387,11 @@ def route_tokens(scores: torch.Tensor, top_k: int, *, token_mask: Optional[torch
     logits to bf16, this function does not."""
     top_k, router = int(top_k), (int(router[0]), float(router[1]), float(router[2]))
     if _is_compiling():
-        idx, gates, counts, losses = torch.ops.tmoe_b200.route_tokens(scores, token_mask, top_k, *router)
+        idx, gates, counts, losses, _ = torch.ops.tmoe_b200.route_tokens(scores, token_mask, top_k, *router)
         return Routing(idx, gates, counts, losses[0], losses[1])
     if scores.requires_grad and torch.is_grad_enabled():
         return Routing(*_RouteTokens.apply(scores, token_mask, top_k, router))
-    idx, gates, counts, losses = _route_forward(scores, token_mask, top_k, router)
+    idx, gates, counts, losses, _ = _route_forward(scores, token_mask, top_k, router)
     return Routing(idx, gates, counts, losses[0], losses[1])
 
 

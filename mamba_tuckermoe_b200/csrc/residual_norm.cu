@@ -24,6 +24,7 @@
 // the two rstd of a row are kept from the forward pass.
 #include "common.cuh"
 #include "kernels.h"
+#include "pair.cuh"
 #include "ptx.cuh"
 
 namespace tmoe {
@@ -38,28 +39,13 @@ constexpr int block_warps(int nv, bool back, bool f32) { return back ? resident_
 constexpr int kMaxTeams = 10;           // teams of several warps in a block (a named barrier each)
 constexpr int kRingBytes = 208 * 1024;
 
-// Two fp32 values worked on by one instruction: the walk is bound by the instructions it issues as much as by memory (80 a element in
-// scalar form), and sm_100 multiplies and adds pairs at the price of one.
-using f2 = unsigned long long;
-__device__ __forceinline__ f2 pair(float lo, float hi) { f2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi)); return r; }
-__device__ __forceinline__ f2 both(float v) { return pair(v, v); }
-__device__ __forceinline__ void split(f2 v, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
-__device__ __forceinline__ f2 mul2(f2 a, f2 b) { f2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
-__device__ __forceinline__ f2 add2(f2 a, f2 b) { f2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
-__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) { f2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
-__device__ __forceinline__ float sum2(f2 v) { float a, b; split(v, a, b); return a + b; }
-
 // sigmoid to a few ulp (the gate is one factor of a sum that is rounded to the storage type).  exp(-g) beyond the range is 0 or infinite,
 // and its reciprocal 1 or 0.
 __device__ __forceinline__ f2 sigmoid2(f2 g) {
   float a, b;
-  split(mul2(g, both(-1.4426950408889634f)), a, b);
-  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(a));
-  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(b));
-  split(add2(pair(a, b), both(1.f)), a, b);
-  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(a));
-  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(b));
-  return pair(a, b);
+  split(mul2(g, both(-kLog2e)), a, b);
+  split(add2(pair(fast_exp2(a), fast_exp2(b)), both(1.f)), a, b);
+  return pair(fast_rcp(a), fast_rcp(b));
 }
 
 __device__ __forceinline__ void cp_async16(void *smem, const void *gmem) {

@@ -22,6 +22,7 @@
 //   ds = dl (rule 0),  dl * sech^2(s / cap) / temp (rule 1)
 #include "common.cuh"
 #include "kernels.h"
+#include "pair.cuh"
 #include "ptx.cuh"
 
 #include <cmath>
@@ -38,11 +39,12 @@ struct RouteArgs {
   const uint8_t *mask;       // [tokens] or nullptr
   int64_t tokens, stride;    // stride: elements between score rows
   int E, k, rule;
-  float cap, inv_cap, inv_temp;
+  float inv_cap, scale;      // logit = scale * tanh(score * inv_cap)
   int32_t *idx;              // [tokens, k]
   float *gates;              // [tokens, k]
   int32_t *counts;           // [E]
   float *losses;             // balance, z, n
+  float *stats;              // [tokens, 2]: largest logit and sum of exp(logit - largest) of a token, or nullptr
   float *part_p;             // [blocks, E]
   int32_t *part_c;           // [blocks, E]
   float *part_zn;            // [blocks, 2]
@@ -51,18 +53,26 @@ struct RouteArgs {
   void *d_scores;            // [tokens, E]
 };
 
-// Selection keys: unsigned order = higher score first, equal scores lower column first; 0 = switched off.
+// Selection keys: unsigned order = higher score first, equal scores lower column first.  Adding zero beforehand makes -0 equal to +0 and
+// every NaN the positive one, which sorts above +inf.  -inf is the lowest key that a score can have and marks an expert that is off.
 template <typename TS> struct Key;
 template <> struct Key<bf16> {
-  using type = uint32_t;
-  __device__ static __forceinline__ uint32_t make(float v, int col) {
-    uint32_t b = __float_as_uint(v) >> 16;
-    if ((b & 0x7fffu) > 0x7f80u) b = 0x7fffu;            // NaN above everything
-    if (b == 0xff80u) return 0u;                         // -inf
-    if (b == 0x8000u) b = 0u;                            // -0 equals +0
-    const uint32_t u = (b & 0x8000u) ? (~b & 0xffffu) : (b | 0x8000u);
-    return (u << 16) | (0xffffu - (uint32_t)col);
+  using type = uint32_t;   // order-preserving bits of the score << 16 | 0xffff - column
+  // the keys of 8 scores, two to a word, in columns col .. col + 7
+  __device__ static __forceinline__ void make(const uint4 &v, int col, uint32_t (&key)[8]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 c = __hadd2(*reinterpret_cast<const __nv_bfloat162 *>(&w[i]), __nv_bfloat162{__ushort_as_bfloat16(0), __ushort_as_bfloat16(0)});
+      const uint32_t u = *reinterpret_cast<const uint32_t *>(&c);
+      uint32_t neg;                                            // 0xffff in the halves whose sign is set
+      asm("prmt.b32 %0, %1, 0, 0xbb99;" : "=r"(neg) : "r"(u));
+      const uint32_t o = u ^ (neg | 0x80008000u);
+      key[2 * i] = (o << 16) + (0xffffu - (uint32_t)(col + 2 * i));
+      key[2 * i + 1] = (o & 0xffff0000u) + (0xffffu - (uint32_t)(col + 2 * i + 1));
+    }
   }
+  __device__ static __forceinline__ bool empty(uint32_t key) { return (key >> 16) <= 0x7fu; }
   __device__ static __forceinline__ int col(uint32_t key) { return (int)(0xffffu - (key & 0xffffu)); }
   __device__ static __forceinline__ float value(uint32_t key) {
     const uint32_t u = key >> 16;
@@ -70,15 +80,13 @@ template <> struct Key<bf16> {
   }
 };
 template <> struct Key<float> {
-  using type = unsigned long long;
-  __device__ static __forceinline__ unsigned long long make(float v, int col) {
-    uint32_t b = __float_as_uint(v);
-    if ((b & 0x7fffffffu) > 0x7f800000u) b = 0x7fffffffu;
-    if (b == 0xff800000u) return 0ull;
-    if (b == 0x80000000u) b = 0u;
-    const uint32_t u = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+  using type = unsigned long long;   // order-preserving bits << 32 | 0xffffffff - column
+  __device__ static __forceinline__ unsigned long long one(float v, int col) {
+    const uint32_t b = __float_as_uint(__fadd_rn(v, 0.f));
+    const uint32_t u = b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
     return ((unsigned long long)u << 32) | (0xffffffffu - (uint32_t)col);
   }
+  __device__ static __forceinline__ bool empty(unsigned long long key) { return (uint32_t)(key >> 32) <= 0x007fffffu; }
   __device__ static __forceinline__ int col(unsigned long long key) { return (int)(0xffffffffu - (uint32_t)key); }
   __device__ static __forceinline__ float value(unsigned long long key) {
     const uint32_t u = (uint32_t)(key >> 32);
@@ -93,11 +101,6 @@ template <int G> struct Slots { static constexpr int N = G <= 2 ? 8 : G == 4 ? 4
 template <int G> __device__ __forceinline__ float group_sum(float v) {
 #pragma unroll
   for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-template <int G> __device__ __forceinline__ float group_max(float v) {
-#pragma unroll
-  for (int o = G / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
 template <int G> __device__ __forceinline__ uint32_t group_max(uint32_t v) {
@@ -120,118 +123,234 @@ template <int G> __device__ __forceinline__ unsigned long long group_max(unsigne
   return v;
 }
 
-// The 8 * NC scores of one lane: columns (c * G + gl) * 8 + q.  Columns beyond E read as -inf.
-template <typename TS, int G, int NC, bool WIDE>
-__device__ __forceinline__ void load_scores(const TS *row, int gl, int E, bool want, float (&s)[NC * 8]) {
-#pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    const int e0 = (c * G + gl) * 8;
+// The 8 scores of one lane in columns e0 .. e0 + 7, as pairs.  What is not there (column, token, masked token) reads as -inf.
+template <typename TS, bool WIDE> struct Chunk;
+template <bool WIDE> struct Chunk<bf16, WIDE> {
+  uint4 v;
+  __device__ __forceinline__ void load(const bf16 *row, int e0, int E, bool want) {
+    v = make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);
     if (WIDE) {
-      if (want && e0 < E) {   // E % 8 == 0
-        if (sizeof(TS) == 2) {
-          const uint4 v = __ldg(reinterpret_cast<const uint4 *>(row + e0));
-          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+      if (want && e0 < E) v = __ldg(reinterpret_cast<const uint4 *>(row + e0));   // E % 8 == 0
+    } else if (want) {
+      uint32_t h[8];
 #pragma unroll
-          for (int q = 0; q < 8; ++q) s[c * 8 + q] = __uint_as_float((q & 1) ? (w[q >> 1] & 0xffff0000u) : (w[q >> 1] << 16));
-        } else {
-          const float4 a = __ldg(reinterpret_cast<const float4 *>(row + e0)), b = __ldg(reinterpret_cast<const float4 *>(row + e0) + 1);
-          const float f[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-          for (int q = 0; q < 8; ++q) s[c * 8 + q] = f[q];
-        }
-      } else {
-#pragma unroll
-        for (int q = 0; q < 8; ++q) s[c * 8 + q] = -INFINITY;
-      }
-    } else {
-#pragma unroll
-      for (int q = 0; q < 8; ++q) s[c * 8 + q] = (want && e0 + q < E) ? to_f32(row[e0 + q]) : -INFINITY;
+      for (int q = 0; q < 8; ++q) h[q] = e0 + q < E ? (uint32_t)__bfloat16_as_ushort(row[e0 + q]) : 0xff80u;
+      v = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
     }
   }
+  __device__ __forceinline__ void keys(int e0, uint32_t (&key)[8]) const { Key<bf16>::make(v, e0, key); }
+  __device__ __forceinline__ f2 get(int j) const {
+    const uint32_t w = j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w;
+    return pair(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  }
+};
+template <bool WIDE> struct Chunk<float, WIDE> {
+  float v[8];
+  __device__ __forceinline__ void load(const float *row, int e0, int E, bool want) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = -INFINITY;
+    if (WIDE) {
+      if (want && e0 < E) {
+        const float4 a = __ldg(reinterpret_cast<const float4 *>(row + e0)), b = __ldg(reinterpret_cast<const float4 *>(row + e0) + 1);
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+      }
+    } else if (want) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        if (e0 + q < E) v[q] = row[e0 + q];
+    }
+  }
+  __device__ __forceinline__ void keys(int e0, unsigned long long (&key)[8]) const {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) key[q] = Key<float>::one(v[q], e0 + q);
+  }
+  __device__ __forceinline__ f2 get(int j) const { return pair(v[2 * j], v[2 * j + 1]); }
+};
+
+// tanh of two values.  Up to 1 in magnitude by the Pade approximant x (945 + 105 x^2 + x^4) / (945 + 420 x^2 + 15 x^4) that Lambert's continued
+// fraction gives (6e-8 off at 1, less below), beyond that by 1 - 2 e / (1 + e) with e = exp(-2|x|), whose error shrinks with e.  NaN stays
+// NaN; the branch is the warp's, and scores seldom reach the cap.
+__device__ __forceinline__ f2 tanh2(f2 x) {
+  const f2 q = mul2(x, x);
+  float da, db, xa, xb;
+  split(fma2(q, fma2(q, both(15.f), both(420.f)), both(945.f)), da, db);
+  f2 t = mul2(mul2(x, fma2(q, add2(q, both(105.f)), both(945.f))), pair(fast_rcp(da), fast_rcp(db)));
+  split(x, xa, xb);
+  const bool fa = fabsf(xa) > 1.f, fb = fabsf(xb) > 1.f;
+  if (__any_sync(0xffffffffu, fa || fb)) {
+    float ta, tb;
+    split(t, ta, tb);
+    const float ea = fast_exp2(fabsf(xa) * (-2.f * kLog2e)), eb = fast_exp2(fabsf(xb) * (-2.f * kLog2e));
+    if (fa) ta = copysignf(1.f - 2.f * ea * fast_rcp(1.f + ea), xa);
+    if (fb) tb = copysignf(1.f - 2.f * eb * fast_rcp(1.f + eb), xb);
+    t = pair(ta, tb);
+  }
+  return t;
+}
+// 1 - tanh^2 at x, given t = tanh(x): from t up to 1, from e beyond, where 1 - t^2 would cancel
+__device__ __forceinline__ f2 sech2(f2 x, f2 t) {
+  f2 r = fma2(mul2(t, both(-1.f)), t, both(1.f));
+  float xa, xb;
+  split(x, xa, xb);
+  const bool fa = fabsf(xa) > 1.f, fb = fabsf(xb) > 1.f;
+  if (__any_sync(0xffffffffu, fa || fb)) {
+    float ra, rb;
+    split(r, ra, rb);
+    const float ea = fast_exp2(fabsf(xa) * (-2.f * kLog2e)), eb = fast_exp2(fabsf(xb) * (-2.f * kLog2e));
+    const float ia = fast_rcp(1.f + ea), ib = fast_rcp(1.f + eb);
+    if (fa) ra = 4.f * ea * ia * ia;
+    if (fb) rb = 4.f * eb * ib * ib;
+    r = pair(ra, rb);
+  }
+  return r;
 }
 
-__device__ __forceinline__ float logit_of(const RouteArgs &a, float s) {
-  return a.rule == 1 ? a.cap * tanhf(s * a.inv_cap) * a.inv_temp : s;
+template <typename K> __device__ __forceinline__ void sort_two(K &a, K &b) {   // larger first
+  const K hi = a > b ? a : b, lo = a > b ? b : a;
+  a = hi; b = lo;
+}
+// The DEPTH largest of 8 keys, sorted, in the first places: all 8 by Batcher's network of 19 exchanges, or the first two by a
+// tournament of pairs.
+template <int DEPTH, typename K> __device__ __forceinline__ void sort_keys(K (&k)[8]) {
+  sort_two(k[0], k[1]); sort_two(k[2], k[3]); sort_two(k[4], k[5]); sort_two(k[6], k[7]);
+  if (DEPTH == 2) {
+#pragma unroll
+    for (int w = 2; w < 8; w *= 2) {
+#pragma unroll
+      for (int i = 0; i < 8; i += 2 * w) {
+        const K lo = k[i] > k[i + w] ? k[i + w] : k[i], second = k[i + 1] > k[i + w + 1] ? k[i + 1] : k[i + w + 1];
+        k[i] = k[i] > k[i + w] ? k[i] : k[i + w];
+        k[i + 1] = lo > second ? lo : second;
+      }
+    }
+    return;
+  }
+  sort_two(k[0], k[2]); sort_two(k[1], k[3]); sort_two(k[4], k[6]); sort_two(k[5], k[7]);
+  sort_two(k[1], k[2]); sort_two(k[5], k[6]);
+  sort_two(k[0], k[4]); sort_two(k[1], k[5]); sort_two(k[2], k[6]); sort_two(k[3], k[7]);
+  sort_two(k[2], k[4]); sort_two(k[3], k[5]);
+  sort_two(k[1], k[2]); sort_two(k[3], k[4]); sort_two(k[5], k[6]);
 }
 
-// G lanes per token, a warp walks over tokens with all its groups; every lane owns the same columns in all of them, so P and the
-// counts are sums in its registers.  Blocks write one row of partial sums each.
-template <typename TS, int G, int NC, bool WIDE>
+// The losses from the whole batch's sums; `dot` = sum_e counts_e * sum_t p[t, e]
+__device__ __forceinline__ void write_losses(const RouteArgs &a, float dot, float z, float n) {
+  const float inv = n > 0.f ? 1.f / n : 0.f;
+  a.losses[0] = (float)a.E * (dot * inv) * (inv / (float)a.k);
+  a.losses[1] = z * inv;
+  a.losses[2] = n;
+}
+
+// G lanes per token, 8 columns of NC chunks each; a warp walks over tokens with all its groups, and every lane owns the same columns in all
+// of them, so P is a sum in its registers; the choices are counted in shared memory (integers: the order of the atomics does not matter).
+// A lane's keys are sorted once, so that a round of the selection is one maximum over the lanes' heads and a shift in the winner's list.
+// Blocks write one row of partial sums each; a block that is alone finishes the losses itself.
+template <typename TS, int G, int NC, int DEPTH, bool WIDE>
 __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_constant__ RouteArgs a) {
   using K = Key<TS>;
-  constexpr int N = NC * 8, SL = Slots<G>::N;          // columns and slots per lane
-  extern __shared__ float sm[];                        // [warps][G * N]: P, then the counts
+  constexpr int N = NC * 8, SL = Slots<G>::N, PER = 32 / G;   // columns and slots per lane, tokens per warp
+  extern __shared__ float sm[];                               // [warps][G * N]
+  __shared__ int hist[G * N];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gl = lane % G, grp = lane / G;
-  constexpr int PER = 32 / G;
-  float acc[N];
-  int cnt[N];
+  ptx::griddep_launch_dependents();
+  for (int i = threadIdx.x; i < G * N; i += kRouteThreads) hist[i] = 0;
+  __syncthreads();
+  f2 acc[N / 2];
 #pragma unroll
-  for (int x = 0; x < N; ++x) { acc[x] = 0.f; cnt[x] = 0; }
+  for (int x = 0; x < N / 2; ++x) acc[x] = both(0.f);
   float zsum = 0.f, nsum = 0.f;
-  for (int64_t t0 = ((int64_t)blockIdx.x * kRouteWarps + warp) * PER; t0 < a.tokens; t0 += (int64_t)gridDim.x * kRouteWarps * PER) {
+  const int64_t step = (int64_t)gridDim.x * kRouteWarps * PER;
+  for (int64_t t0 = ((int64_t)blockIdx.x * kRouteWarps + warp) * PER; t0 < a.tokens; t0 += step) {
     const int64_t t = t0 + grp;
     const bool here = t < a.tokens;
     const bool want = here && (!a.mask || a.mask[t]);
-    float s[N];
-    load_scores<TS, G, NC, WIDE>((const TS *)a.scores + t * a.stride, gl, a.E, want, s);
-    typename K::type key[N];
+    Chunk<TS, WIDE> s[NC];
+    typename K::type key[NC][8];
 #pragma unroll
-    for (int x = 0; x < N; ++x) key[x] = K::make(s[x], ((x / 8) * G + gl) * 8 + x % 8);
-    typename K::type mine[SL];
-    float top = 0.f;
-    bool live = false;
-#pragma unroll
-    for (int i = 0; i < SL; ++i) mine[i] = 0;
+    for (int c = 0; c < NC; ++c) {
+      s[c].load((const TS *)a.scores + t * a.stride, (c * G + gl) * 8, a.E, want);
+      s[c].keys((c * G + gl) * 8, key[c]);
+      sort_keys<DEPTH>(key[c]);
+    }
+    typename K::type mine[SL], first = 0;
 #pragma unroll
     for (int i = 0; i < SL; ++i) {
+      mine[i] = 0;
       const int last = min(G, a.k - i * G);
 #pragma unroll 1
       for (int jj = 0; jj < last; ++jj) {
-        typename K::type m = key[0];
+        typename K::type m = key[0][0];
 #pragma unroll
-        for (int x = 1; x < N; ++x) m = key[x] > m ? key[x] : m;
+        for (int c = 1; c < NC; ++c) m = key[c][0] > m ? key[c][0] : m;
         m = group_max<G>(m);
-        if (i == 0 && jj == 0) { live = m != 0; top = live ? logit_of(a, K::value(m)) : 0.f; }
+        if (i == 0 && jj == 0) first = m;
         if (gl == jj) mine[i] = m;
 #pragma unroll
-        for (int x = 0; x < N; ++x) key[x] = key[x] == m ? 0 : key[x];
+        for (int c = 0; c < NC; ++c) {
+          const bool won = key[c][0] == m;
+#pragma unroll
+          for (int q = 0; q + 1 < DEPTH; ++q) key[c][q] = won ? key[c][q + 1] : key[c][q];
+          key[c][DEPTH - 1] = won ? 0 : key[c][DEPTH - 1];
+        }
       }
     }
-    float den = 0.f;
+    const bool live = !K::empty(first);
+    float ta, tb;
+    split(a.rule == 1 ? mul2(tanh2(mul2(both(K::value(first)), both(a.inv_cap))), both(a.scale)) : both(K::value(first)), ta, tb);
+    const float top = live ? ta : 0.f;
+    f2 ex[N / 2], sum = both(0.f);
 #pragma unroll
-    for (int x = 0; x < N; ++x) {
-      const bool on = s[x] != -INFINITY;
-      cnt[x] += (on && key[x] == 0) ? 1 : 0;
-      s[x] = on ? expf(logit_of(a, s[x]) - top) : 0.f;
-      den += s[x];
+    for (int x = 0; x < N / 2; ++x) {
+      const f2 v = s[x / 4].get(x % 4);
+      f2 l = v;
+      if (a.rule == 1) l = mul2(tanh2(mul2(v, both(a.inv_cap))), both(a.scale));
+      float la, lb;
+      split(mul2(add2(l, both(-top)), both(kLog2e)), la, lb);   // (the difference first: exact for what matters, whatever the scores' size)
+      float ea = fast_exp2(la), eb = fast_exp2(lb);
+      if (a.rule == 1) {   // the cap makes -inf a number again
+        float va, vb;
+        split(v, va, vb);
+        ea = va == -INFINITY ? 0.f : ea;
+        eb = vb == -INFINITY ? 0.f : eb;
+      }
+      ex[x] = pair(ea, eb);
+      sum = add2(sum, ex[x]);
     }
-    den = group_sum<G>(den);
+    const float den = group_sum<G>(sum2(sum));
     const float inv = live ? 1.f / den : 0.f;
     if (live) {
 #pragma unroll
-      for (int x = 0; x < N; ++x) acc[x] = fmaf(s[x], inv, acc[x]);
+      for (int x = 0; x < N / 2; ++x) acc[x] = fma2(ex[x], both(inv), acc[x]);
       if (gl == 0) {
         const float lse = top + logf(den);
         zsum = fmaf(lse, lse, zsum);
         nsum += 1.f;
+        if (a.stats) reinterpret_cast<float2 *>(a.stats)[t] = make_float2(top, den);
       }
     }
-    float g[SL], sum = 0.f;
+    float g[SL], total = 0.f;
 #pragma unroll
     for (int i = 0; i < SL; ++i) {
-      g[i] = mine[i] != 0 ? expf(logit_of(a, K::value(mine[i])) - top) : 0.f;
-      if (a.rule == 1) g[i] *= inv;
-      sum += g[i];
+      g[i] = 0.f;
+      if (i * G < a.k) {   // (uniform)
+        float va, vb;
+        split(a.rule == 1 ? mul2(tanh2(mul2(both(K::value(mine[i])), both(a.inv_cap))), both(a.scale)) : both(K::value(mine[i])), va, vb);
+        if (!K::empty(mine[i])) g[i] = fast_exp2((va - top) * kLog2e);
+        if (a.rule == 1) g[i] *= inv;
+        total += g[i];
+      }
     }
-    sum = group_sum<G>(sum);
-    if (a.rule == 1) sum += 1e-6f;
+    total = group_sum<G>(total);
+    if (a.rule == 1) total += 1e-6f;
+    const float over = live ? 1.f / total : 0.f;
     if (here) {
 #pragma unroll
       for (int i = 0; i < SL; ++i) {
         const int j = i * G + gl;
         if (j < a.k) {
-          a.idx[t * a.k + j] = mine[i] != 0 ? K::col(mine[i]) : -1;
-          a.gates[t * a.k + j] = mine[i] != 0 ? g[i] / sum : 0.f;
+          const bool full = !K::empty(mine[i]);
+          a.idx[t * a.k + j] = full ? K::col(mine[i]) : -1;
+          a.gates[t * a.k + j] = full ? g[i] * over : 0.f;
+          if (full) atomicAdd(&hist[K::col(mine[i])], 1);
         }
       }
     }
@@ -239,184 +358,236 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_const
   // the block's sums: groups of a warp by shuffles, then the warps in order
 #pragma unroll
   for (int x = 0; x < N; ++x) {
+    float lo, hi;
+    split(acc[x / 2], lo, hi);
+    float v = (x & 1) ? hi : lo;
 #pragma unroll
-    for (int o = G; o < 32; o <<= 1) {
-      acc[x] += __shfl_xor_sync(0xffffffffu, acc[x], o);
-      cnt[x] += __shfl_xor_sync(0xffffffffu, cnt[x], o);
-    }
-    if (grp == 0) sm[warp * (G * N) + ((x / 8) * G + gl) * 8 + x % 8] = acc[x];
+    for (int o = G; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (grp == 0) sm[warp * (G * N) + ((x / 8) * G + gl) * 8 + x % 8] = v;
   }
-  __shared__ float szn[kRouteWarps][2];
+  __shared__ float szn[kRouteWarps][3];
   zsum = warp_sum(zsum); nsum = warp_sum(nsum);
   if (lane == 0) { szn[warp][0] = zsum; szn[warp][1] = nsum; }
   __syncthreads();
+  const bool alone = gridDim.x == 1;
+  float dot = 0.f;
   for (int e = threadIdx.x; e < a.E; e += kRouteThreads) {
     float p = 0.f;
 #pragma unroll
     for (int w = 0; w < kRouteWarps; ++w) p += sm[w * (G * N) + e];
-    a.part_p[(int64_t)blockIdx.x * a.E + e] = p;
+    if (alone) {
+      a.counts[e] = hist[e];
+      dot = fmaf((float)hist[e], p, dot);
+    } else {
+      a.part_p[(int64_t)blockIdx.x * a.E + e] = p;
+      a.part_c[(int64_t)blockIdx.x * a.E + e] = hist[e];
+    }
   }
-  __syncthreads();
-  int *si = reinterpret_cast<int *>(sm);
-  if (grp == 0) {
-#pragma unroll
-    for (int x = 0; x < N; ++x) si[warp * (G * N) + ((x / 8) * G + gl) * 8 + x % 8] = cnt[x];
+  if (alone) {
+    dot = warp_sum(dot);
+    if (lane == 0) szn[warp][2] = dot;
+    __syncthreads();
   }
-  __syncthreads();
-  for (int e = threadIdx.x; e < a.E; e += kRouteThreads) {
-    int c = 0;
+  if (threadIdx.x == 0) {
+    float z = 0.f, n = 0.f, d = 0.f;
 #pragma unroll
-    for (int w = 0; w < kRouteWarps; ++w) c += si[w * (G * N) + e];
-    a.part_c[(int64_t)blockIdx.x * a.E + e] = c;
-  }
-  if (threadIdx.x < 2) {
-    float v = 0.f;
-#pragma unroll
-    for (int w = 0; w < kRouteWarps; ++w) v += szn[w][threadIdx.x];
-    a.part_zn[blockIdx.x * 2 + threadIdx.x] = v;
+    for (int w = 0; w < kRouteWarps; ++w) { z += szn[w][0]; n += szn[w][1]; d += alone ? szn[w][2] : 0.f; }
+    if (alone) {
+      write_losses(a, d, z, n);
+    } else {
+      a.part_zn[blockIdx.x * 2] = z;
+      a.part_zn[blockIdx.x * 2 + 1] = n;
+    }
   }
 }
 
-// Sums the blocks' rows in order: counts, and the two losses.  One block.
-__global__ void __launch_bounds__(1024) route_losses_kernel(const __grid_constant__ RouteArgs a, int blocks) {
-  __shared__ float red[32];
+// Sums the blocks' rows in a fixed order: counts, and the two losses.  One cluster of 8 blocks (one block alone took 45 us at 296 rows);
+// each takes an eighth of the columns, `width` threads side by side on them and the others on other rows, and block 0 puts the eight
+// parts of the balance loss together.
+constexpr int kLossBlocks = 8, kLossThreads = 512;
+__global__ void __launch_bounds__(kLossThreads) route_losses_kernel(const __grid_constant__ RouteArgs a, int blocks, int width) {
+  __shared__ float sp[kLossThreads];
+  __shared__ int sc[kLossThreads];
+  __shared__ float parts[kLossBlocks];
+  __shared__ float red[kLossThreads / 32][3];
+  ptx::griddep_wait();
+  ptx::cluster_arrive();   // block 0 runs before anything is stored to its shared memory
+  ptx::cluster_wait();
+  const int rank = blockIdx.x, per = (a.E + kLossBlocks - 1) / kLossBlocks, e0 = rank * per;
+  const int slices = kLossThreads / width, col = threadIdx.x % width, slice = threadIdx.x / width;
   float dot = 0.f;
-  for (int e = threadIdx.x; e < a.E; e += 1024) {
-    float p = 0.f; int c = 0;
-    for (int b = 0; b < blocks; ++b) { p += a.part_p[(int64_t)b * a.E + e]; c += a.part_c[(int64_t)b * a.E + e]; }
-    a.counts[e] = c;
-    dot = fmaf((float)c, p, dot);
+  for (int c0 = 0; c0 < per; c0 += width) {
+    const int e = e0 + c0 + col;
+    const bool in = c0 + col < per && e < a.E && slice < slices;
+    float p = 0.f;
+    int c = 0;
+    if (in) {
+#pragma unroll 4
+      for (int b = slice; b < blocks; b += slices) {
+        p += a.part_p[(int64_t)b * a.E + e];
+        c += a.part_c[(int64_t)b * a.E + e];
+      }
+    }
+    sp[threadIdx.x] = p; sc[threadIdx.x] = c;
+    __syncthreads();
+    for (int n = slices / 2; n > 0; n >>= 1) {   // slices is a power of two
+      if (slice < n) {
+        sp[threadIdx.x] += sp[threadIdx.x + n * width];
+        sc[threadIdx.x] += sc[threadIdx.x + n * width];
+      }
+      __syncthreads();
+    }
+    if (in && slice == 0) {
+      a.counts[e] = sc[threadIdx.x];
+      dot = fmaf((float)sc[threadIdx.x], sp[threadIdx.x], dot);
+    }
+    __syncthreads();
+  }
+  float z = 0.f, n = 0.f;
+  if (rank == 0) {
+    for (int b = threadIdx.x; b < blocks; b += kLossThreads) { z += a.part_zn[2 * b]; n += a.part_zn[2 * b + 1]; }
+    z = warp_sum(z);
+    n = warp_sum(n);
   }
   dot = warp_sum(dot);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = dot;
+  if ((threadIdx.x & 31) == 0) { red[threadIdx.x >> 5][0] = dot; red[threadIdx.x >> 5][1] = z; red[threadIdx.x >> 5][2] = n; }
   __syncthreads();
   if (threadIdx.x == 0) {
-    float z = 0.f, n = 0.f;
-    for (int b = 0; b < blocks; ++b) { z += a.part_zn[2 * b]; n += a.part_zn[2 * b + 1]; }
     dot = 0.f;
-    for (int w = 0; w < 32; ++w) dot += red[w];
-    const float inv = n > 0.f ? 1.f / n : 0.f;
-    a.losses[0] = (float)a.E * (dot * inv) * (inv / (float)a.k);
-    a.losses[1] = z * inv;
-    a.losses[2] = n;
+    for (int w = 0; w < kLossThreads / 32; ++w) dot += red[w][0];
+    ptx::st_cluster_u32(ptx::mapa_u32(ptx::smem_u32(&parts[rank]), 0), __float_as_uint(dot));
+  }
+  __syncthreads();
+  ptx::cluster_arrive();
+  ptx::cluster_wait();
+  if (rank == 0 && threadIdx.x == 0) {
+    dot = z = n = 0.f;
+    for (int r = 0; r < kLossBlocks; ++r) dot += parts[r];
+    for (int w = 0; w < kLossThreads / 32; ++w) { z += red[w][1]; n += red[w][2]; }
+    write_losses(a, dot, z, n);
   }
 }
 
+// p comes from the kept largest logit and sum, so a token needs one pass over its row.  The gates' parts of the gradient go through a row of shared memory
+// per token: the lanes that hold slots put them at their columns, and every lane picks up its own eight.
 template <typename TS, int G, int NC, bool WIDE>
 __global__ void __launch_bounds__(kRouteThreads) route_backward_kernel(const __grid_constant__ RouteArgs a) {
   constexpr int N = NC * 8, SL = Slots<G>::N, PER = 32 / G;
+  extern __shared__ __align__(16) float sm[];   // [warps][PER][G * N]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gl = lane % G, grp = lane / G;
+  float *row = sm + (warp * PER + grp) * (G * N);
+  for (int i = gl; i < G * N; i += G) row[i] = 0.f;
+  __syncwarp();
   const float n = a.losses[2], inv_n = n > 0.f ? 1.f / n : 0.f;
   const float z2 = a.d_z ? *a.d_z * 2.f * inv_n : 0.f;
   const float bal = a.d_balance ? *a.d_balance * ((float)a.E * inv_n) * (inv_n / (float)a.k) : 0.f;
-  float A[N];
+  f2 A[N / 2];
 #pragma unroll
-  for (int x = 0; x < N; ++x) {
-    const int col = ((x / 8) * G + gl) * 8 + x % 8;
-    A[x] = col < a.E ? bal * (float)a.counts[col] : 0.f;
+  for (int x = 0; x < N / 2; ++x) {
+    const int col = ((x / 4) * G + gl) * 8 + x % 4 * 2;
+    A[x] = pair(col < a.E ? bal * (float)a.counts[col] : 0.f, col + 1 < a.E ? bal * (float)a.counts[col + 1] : 0.f);
   }
-  for (int64_t t0 = ((int64_t)blockIdx.x * kRouteWarps + warp) * PER; t0 < a.tokens; t0 += (int64_t)gridDim.x * kRouteWarps * PER) {
+  const int64_t step = (int64_t)gridDim.x * kRouteWarps * PER;
+  for (int64_t t0 = ((int64_t)blockIdx.x * kRouteWarps + warp) * PER; t0 < a.tokens; t0 += step) {
     const int64_t t = t0 + grp;
     const bool here = t < a.tokens;
     const bool want = here && (!a.mask || a.mask[t]);
-    float s[N], th[N];
-    load_scores<TS, G, NC, WIDE>((const TS *)a.scores + t * a.stride, gl, a.E, want, s);
-    float top = -INFINITY;
-    bool any = false;
+    Chunk<TS, WIDE> s[NC];
 #pragma unroll
-    for (int x = 0; x < N; ++x) {
-      const bool on = s[x] != -INFINITY;
-      any |= on;
-      if (a.rule == 1) {
-        // sech^2 from exp(-2|s/cap|): no cancellation where the cap saturates
-        const float e = expf(-2.f * fabsf(s[x] * a.inv_cap)), d = 1.f / (1.f + e);
-        th[x] = on ? 4.f * e * d * d * a.inv_temp : 0.f;
-        s[x] = on ? logit_of(a, s[x]) : -INFINITY;
-      } else {
-        th[x] = on ? 1.f : 0.f;
-      }
-      top = fmaxf(top, s[x]);
-    }
-    top = group_max<G>(top);
-    const bool live = (__ballot_sync(0xffffffffu, any) >> (grp * G) & (G == 32 ? 0xffffffffu : ((1u << G) - 1u))) != 0u;
-    float den = 0.f, dot = 0.f;
-#pragma unroll
-    for (int x = 0; x < N; ++x) {
-      s[x] = s[x] != -INFINITY ? expf(s[x] - top) : 0.f;
-      den += s[x];
-    }
-    den = group_sum<G>(den);
-    const float inv = live ? 1.f / den : 0.f;
-    const float lse = live ? top + logf(den) : 0.f;
-#pragma unroll
-    for (int x = 0; x < N; ++x) {
-      s[x] *= inv;
-      dot = fmaf(s[x], A[x], dot);
-    }
-    dot = group_sum<G>(dot);
-    // the gates' part: lane j % G holds slot j
+    for (int c = 0; c < NC; ++c) s[c].load((const TS *)a.scores + t * a.stride, (c * G + gl) * 8, a.E, want);
+    // slots: lane j % G holds slot j
     int col[SL];
-    float val[SL], inner = 0.f, total = 0.f;
+    float val[SL], dg[SL], inner = 0.f, total = 0.f;
 #pragma unroll
     for (int i = 0; i < SL; ++i) {
       const int j = i * G + gl;
-      col[i] = -1; val[i] = 0.f;
+      col[i] = -1; val[i] = dg[i] = 0.f;
       if (a.d_gates && want && j < a.k) {
         col[i] = a.idx[t * a.k + j];
+        if ((unsigned)col[i] >= (unsigned)a.E) col[i] = -1;
         if (col[i] >= 0) {
-          const float g = a.gates[t * a.k + j], dg = a.d_gates[t * a.k + j];
-          inner = fmaf(g, dg, inner);
-          total += g;
-          val[i] = g;
+          val[i] = a.gates[t * a.k + j];
+          dg[i] = a.d_gates[t * a.k + j];
+          inner = fmaf(val[i], dg[i], inner);
+          total += val[i];
         }
       }
     }
-    inner = group_sum<G>(inner);
-    total = group_sum<G>(total);
+    // a token that counts has a chosen expert in slot 0, and statistics
+    const bool live = want && a.idx[t * a.k] >= 0;
+    const float2 stat = live ? reinterpret_cast<const float2 *>(a.stats)[t] : make_float2(0.f, 1.f);
+    const float lse = stat.x + logf(stat.y), inv = 1.f / stat.y;
+    f2 p[N / 2], th[N / 2], dot2 = both(0.f);
 #pragma unroll
-    for (int i = 0; i < SL; ++i) {
-      const int j = i * G + gl;
-      if (col[i] >= 0) val[i] *= a.d_gates[t * a.k + j] - inner;
+    for (int x = 0; x < N / 2; ++x) {
+      const f2 v = s[x / 4].get(x % 4);
+      f2 l = v;
+      th[x] = both(1.f);
+      if (a.rule == 1) {
+        const f2 y = mul2(v, both(a.inv_cap)), t1 = tanh2(y);
+        th[x] = mul2(sech2(y, t1), both(a.scale * a.inv_cap));
+        l = mul2(t1, both(a.scale));
+      }
+      float la, lb, va, vb;
+      split(mul2(add2(l, both(-stat.x)), both(kLog2e)), la, lb);
+      split(v, va, vb);
+      p[x] = mul2(pair(va == -INFINITY ? 0.f : fast_exp2(la), vb == -INFINITY ? 0.f : fast_exp2(lb)), both(inv));
+      dot2 = fma2(p[x], A[x], dot2);
     }
-    const float base = z2 * lse - dot - (a.rule == 1 ? inner * (1.f - total) : 0.f);
-#pragma unroll
-    for (int x = 0; x < N; ++x) s[x] *= A[x] + base;
+    const float dot = group_sum<G>(sum2(dot2));
+    float base = z2 * lse - dot;
     if (a.d_gates) {
+      inner = group_sum<G>(inner);
+      if (a.rule == 1) base -= inner * (1.f - group_sum<G>(total));
 #pragma unroll
-      for (int i = 0; i < SL; ++i) {
-        const int last = min(G, a.k - i * G);
-#pragma unroll 1
-        for (int jj = 0; jj < last; ++jj) {
-          const int cj = __shfl_sync(0xffffffffu, col[i], grp * G + jj);
-          const float vj = __shfl_sync(0xffffffffu, val[i], grp * G + jj);
-#pragma unroll
-          for (int x = 0; x < N; ++x) s[x] += cj == ((x / 8) * G + gl) * 8 + x % 8 ? vj : 0.f;
-        }
-      }
+      for (int i = 0; i < SL; ++i)
+        if (col[i] >= 0) row[col[i]] = val[i] * (dg[i] - inner);
+      __syncwarp();
     }
+    TS *dst = (TS *)a.d_scores + t * a.E;
 #pragma unroll
-    for (int x = 0; x < N; ++x) s[x] = th[x] != 0.f ? s[x] * th[x] : 0.f;
-    if (here) {
-      TS *dst = (TS *)a.d_scores + t * a.E;
+    for (int c = 0; c < NC; ++c) {
+      const int e0 = (c * G + gl) * 8;
+      f2 d[4];
+      float4 r0 = make_float4(0.f, 0.f, 0.f, 0.f), r1 = r0;
+      if (a.d_gates) { r0 = *reinterpret_cast<const float4 *>(row + e0); r1 = *reinterpret_cast<const float4 *>(row + e0 + 4); }
+      d[0] = pair(r0.x, r0.y); d[1] = pair(r0.z, r0.w); d[2] = pair(r1.x, r1.y); d[3] = pair(r1.z, r1.w);
+      float f[8];
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const int e0 = (c * G + gl) * 8;
+      for (int j = 0; j < 4; ++j) {
+        const int x = c * 4 + j;
+        d[j] = mul2(fma2(p[x], add2(A[x], both(base)), d[j]), th[x]);
+        split(d[j], f[2 * j], f[2 * j + 1]);
+        // an expert that is off, a token that does not count: no gradient (sech^2 of -inf is 0 by itself; rule 0 needs the test)
+        float va, vb;
+        split(s[c].get(j), va, vb);
+        if (va == -INFINITY) f[2 * j] = 0.f;
+        if (vb == -INFINITY) f[2 * j + 1] = 0.f;
+      }
+      if (here) {
         if (WIDE) {
           if (e0 < a.E) {
             if (sizeof(TS) == 2) {
-              *reinterpret_cast<uint4 *>(dst + e0) = make_uint4(pack_bf16x2(s[c * 8], s[c * 8 + 1]), pack_bf16x2(s[c * 8 + 2], s[c * 8 + 3]),
-                                                                pack_bf16x2(s[c * 8 + 4], s[c * 8 + 5]), pack_bf16x2(s[c * 8 + 6], s[c * 8 + 7]));
+              *reinterpret_cast<uint4 *>(dst + e0) =
+                  make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
             } else {
-              reinterpret_cast<float4 *>(dst + e0)[0] = make_float4(s[c * 8], s[c * 8 + 1], s[c * 8 + 2], s[c * 8 + 3]);
-              reinterpret_cast<float4 *>(dst + e0)[1] = make_float4(s[c * 8 + 4], s[c * 8 + 5], s[c * 8 + 6], s[c * 8 + 7]);
+              reinterpret_cast<float4 *>(dst + e0)[0] = make_float4(f[0], f[1], f[2], f[3]);
+              reinterpret_cast<float4 *>(dst + e0)[1] = make_float4(f[4], f[5], f[6], f[7]);
             }
           }
         } else {
 #pragma unroll
           for (int q = 0; q < 8; ++q)
-            if (e0 + q < a.E) dst[e0 + q] = from_f32<TS>(s[c * 8 + q]);
+            if (e0 + q < a.E) dst[e0 + q] = from_f32<TS>(f[q]);
         }
       }
+    }
+    if (a.d_gates) {
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < SL; ++i)
+        if (col[i] >= 0) row[col[i]] = 0.f;
+      __syncwarp();
     }
   }
 }
@@ -428,7 +599,7 @@ int lanes_per_token(int E) {
 }
 int route_blocks(int64_t tokens, int E, int sms) {
   const int64_t per = kRouteWarps * (32 / lanes_per_token(E));
-  const int64_t want = (tokens + per - 1) / per, cap = (int64_t)sms * 2;
+  const int64_t want = (tokens + per - 1) / per, cap = (int64_t)sms * 3;
   return (int)(want < cap ? want : cap);
 }
 
@@ -453,8 +624,8 @@ RouteArgs route_args(const tmoe_route_t &p) {
   RouteArgs a{};
   a.scores = p.scores; a.mask = p.token_mask; a.tokens = p.tokens; a.stride = p.scores_stride;
   a.E = p.n_experts; a.k = p.top_k; a.rule = p.router_mode;
-  a.cap = a.inv_cap = a.inv_temp = 1.f;
-  if (a.rule == 1) { a.cap = p.router_cap; a.inv_cap = 1.f / p.router_cap; a.inv_temp = 1.f / p.router_temperature; }
+  a.scale = a.inv_cap = 1.f;
+  if (a.rule == 1) { a.inv_cap = 1.f / p.router_cap; a.scale = p.router_cap / p.router_temperature; }
   return a;
 }
 
@@ -479,14 +650,16 @@ bool route_wide(const tmoe_route_t &p, const void *d_scores) {
 
 template <typename TS>
 void launch_route(const RouteArgs &a, bool wide, int blocks, cudaStream_t st) {
-#define TMOE_RT(TS_, G, NC, W) route_kernel<TS_, G, NC, W><<<blocks, kRouteThreads, kRouteWarps * G * NC * 8 * 4, st>>>(a)
+#define TMOE_RT(TS_, G, NC, W)                                                                                          \
+  (a.k <= 2 ? (void)route_kernel<TS_, G, NC, 2, W><<<blocks, kRouteThreads, kRouteWarps * G * NC * 8 * 4, st>>>(a)      \
+            : (void)route_kernel<TS_, G, NC, 8, W><<<blocks, kRouteThreads, kRouteWarps * G * NC * 8 * 4, st>>>(a))
   if (wide) TMOE_ROUTE_G(TMOE_RT, TS, true);
   else TMOE_ROUTE_G(TMOE_RT, TS, false);
 #undef TMOE_RT
 }
 template <typename TS>
 void launch_route_backward(const RouteArgs &a, bool wide, int blocks, cudaStream_t st) {
-#define TMOE_RTB(TS_, G, NC, W) route_backward_kernel<TS_, G, NC, W><<<blocks, kRouteThreads, 0, st>>>(a)
+#define TMOE_RTB(TS_, G, NC, W) route_backward_kernel<TS_, G, NC, W><<<blocks, kRouteThreads, kRouteWarps * 32 * NC * 8 * 4, st>>>(a)
   if (wide) TMOE_ROUTE_G(TMOE_RTB, TS, true);
   else TMOE_ROUTE_G(TMOE_RTB, TS, false);
 #undef TMOE_RTB
@@ -508,7 +681,7 @@ int64_t tmoe_route_workspace_bytes(const tmoe_route_t *p) {
   return route_ws(p->tokens ? route_blocks(p->tokens, p->n_experts, 160) : 1, p->n_experts);
 }
 
-int tmoe_route_tokens(const tmoe_route_t *p, int32_t *idx, float *gates, int32_t *counts, float *losses, void *workspace,
+int tmoe_route_tokens(const tmoe_route_t *p, int32_t *idx, float *gates, int32_t *counts, float *losses, float *stats, void *workspace,
                       int64_t workspace_bytes, void *stream) {
   int rc = check_route(p);
   if (rc) return rc;
@@ -522,13 +695,14 @@ int tmoe_route_tokens(const tmoe_route_t *p, int32_t *idx, float *gates, int32_t
   if ((reinterpret_cast<uintptr_t>(idx) | reinterpret_cast<uintptr_t>(gates) | reinterpret_cast<uintptr_t>(counts) |
        reinterpret_cast<uintptr_t>(losses)) & 3)
     return TMOE_ERR_ALIGN;
+  if (reinterpret_cast<uintptr_t>(stats) & 7) return TMOE_ERR_ALIGN;
   if (reinterpret_cast<uintptr_t>(workspace) & 15) return TMOE_ERR_ALIGN;
   const int sms = current_device_sms();
   if (sms <= 0) return TMOE_ERR_CUDA;
   const int blocks = route_blocks(p->tokens, p->n_experts, sms < 160 ? sms : 160);
   if (workspace_bytes < route_ws(blocks, p->n_experts)) return TMOE_ERR_WORKSPACE;
   RouteArgs a = route_args(*p);
-  a.idx = idx; a.gates = gates; a.counts = counts; a.losses = losses;
+  a.idx = idx; a.gates = gates; a.counts = counts; a.losses = losses; a.stats = stats;
   char *ws = reinterpret_cast<char *>(workspace);
   const int64_t one = align_up((int64_t)blocks * a.E * 4, 256);
   a.part_p = reinterpret_cast<float *>(ws);
@@ -539,28 +713,33 @@ int tmoe_route_tokens(const tmoe_route_t *p, int32_t *idx, float *gates, int32_t
   else launch_route<bf16>(a, wide, blocks, st);
   count_launch();
   if ((rc = launch_status())) return rc;
-  route_losses_kernel<<<1, 1024, 0, st>>>(a, blocks);
+  if (blocks == 1) return TMOE_OK;
+  const int per = (a.E + kLossBlocks - 1) / kLossBlocks;
+  int width = 1;
+  while (width < per && width < 64) width *= 2;
+  rc = cuda_ok(launch_pdl_cluster(route_losses_kernel, dim3(kLossBlocks), dim3(kLossThreads), 0, st, kLossBlocks, a, blocks, width));
   count_launch();
-  return launch_status();
+  return rc;
 }
 
 int tmoe_route_tokens_backward(const tmoe_route_t *p, const int32_t *idx, const float *gates, const int32_t *counts,
-                               const float *losses, const float *d_gates, const float *d_balance, const float *d_z, void *d_scores,
-                               void *stream) {
+                               const float *losses, const float *stats, const float *d_gates, const float *d_balance,
+                               const float *d_z, void *d_scores, void *stream) {
   int rc = check_route(p);
   if (rc) return rc;
   if (p->tokens == 0) return TMOE_OK;
-  if (!idx || !gates || !counts || !losses || !d_scores) return TMOE_ERR_NULL;
+  if (!idx || !gates || !counts || !losses || !stats || !d_scores) return TMOE_ERR_NULL;
   if ((reinterpret_cast<uintptr_t>(idx) | reinterpret_cast<uintptr_t>(gates) | reinterpret_cast<uintptr_t>(counts) |
        reinterpret_cast<uintptr_t>(losses) | reinterpret_cast<uintptr_t>(d_gates) | reinterpret_cast<uintptr_t>(d_balance) |
        reinterpret_cast<uintptr_t>(d_z)) & 3)
     return TMOE_ERR_ALIGN;
-  if (reinterpret_cast<uintptr_t>(d_scores) & (p->dtype == TMOE_F32 ? 3 : 1)) return TMOE_ERR_ALIGN;
+  if ((reinterpret_cast<uintptr_t>(d_scores) & (p->dtype == TMOE_F32 ? 3 : 1)) || (reinterpret_cast<uintptr_t>(stats) & 7)) return TMOE_ERR_ALIGN;
   const int sms = current_device_sms();
   if (sms <= 0) return TMOE_ERR_CUDA;
   RouteArgs a = route_args(*p);
   a.idx = const_cast<int32_t *>(idx); a.gates = const_cast<float *>(gates); a.counts = const_cast<int32_t *>(counts);
   a.losses = const_cast<float *>(losses);
+  a.stats = const_cast<float *>(stats);
   a.d_gates = d_gates; a.d_balance = d_balance; a.d_z = d_z; a.d_scores = d_scores;
   const bool wide = route_wide(*p, d_scores);
   const int64_t per = kRouteWarps * (32 / lanes_per_token(a.E)), want = (a.tokens + per - 1) / per;

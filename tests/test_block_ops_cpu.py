@@ -74,27 +74,27 @@ def route(**kw):
 ])
 def test_route_refusals(kw, code):
     lib, p = _lib.load(), route(**kw)
-    assert lib.tmoe_route_tokens(C.byref(p), P, P, P, P, P, 1 << 20, None) == code
+    assert lib.tmoe_route_tokens(C.byref(p), P, P, P, P, P, P, 1 << 20, None) == code
     assert lib.tmoe_route_workspace_bytes(C.byref(p)) == code
-    assert lib.tmoe_route_tokens_backward(C.byref(p), P, P, P, P, P, P, P, P, None) == code
+    assert lib.tmoe_route_tokens_backward(C.byref(p), P, P, P, P, P, P, P, P, P, None) == code
 
 
 def test_route_pointers():
     lib, p = _lib.load(), route()
     assert lib.tmoe_route_workspace_bytes(C.byref(p)) > 0
     assert lib.tmoe_route_workspace_bytes(None) == NULL
-    for i in range(5):
-        args = [P] * 5
+    for i in (0, 1, 2, 3, 5):                                                     # stats (4) is optional
+        args = [P] * 6
         args[i] = None
         assert lib.tmoe_route_tokens(C.byref(p), *args, 1 << 20, None) == NULL
-    assert lib.tmoe_route_tokens(C.byref(p), P + 2, P, P, P, P, 1 << 20, None) == ALIGN
-    assert lib.tmoe_route_tokens(C.byref(p), P, P, P, P, P + 4, 1 << 20, None) == ALIGN
-    for i in (0, 1, 2, 3, 7):
-        args = [P] * 8
+    assert lib.tmoe_route_tokens(C.byref(p), P + 2, P, P, P, P, P, 1 << 20, None) == ALIGN
+    assert lib.tmoe_route_tokens(C.byref(p), P, P, P, P, None, P + 4, 1 << 20, None) == ALIGN
+    for i in (0, 1, 2, 3, 4, 8):
+        args = [P] * 9
         args[i] = None
         assert lib.tmoe_route_tokens_backward(C.byref(p), *args, None) == NULL
-    assert lib.tmoe_route_tokens_backward(C.byref(p), P, P, P, P, P + 2, P, P, P, None) == ALIGN
-    assert lib.tmoe_route_tokens_backward(C.byref(route(tokens=0)), P, P, P, P, P, P, P, P, None) == 0
+    assert lib.tmoe_route_tokens_backward(C.byref(p), P, P, P, P, P, P + 2, P, P, P, None) == ALIGN
+    assert lib.tmoe_route_tokens_backward(C.byref(route(tokens=0)), P, P, P, P, P, P, P, P, P, None) == 0
 
 
 def coef(**kw):
@@ -148,8 +148,8 @@ def test_fake_operators_give_shapes_without_a_gpu():
         assert out.shape == normed.shape == y.shape and out.dtype == torch.float32 and normed.dtype == torch.bfloat16 and rstd.shape == (2, 10)
         g = torch.ops.tmoe_b200.residual_norm_backward(y, res, None, w, None, w, 1e-5, 1e-5, rstd, out, normed)
         assert [t.shape for t in g] == [y.shape, res.shape, w.shape, w.shape]
-        idx, gates, counts, losses = torch.ops.tmoe_b200.route_tokens(torch.empty(3, 7, 40), None, 2, 0, 10.0, 0.5)
-        assert idx.shape == gates.shape == (3, 7, 2) and idx.dtype == counts.dtype == torch.int32 and counts.shape == (40,) and losses.shape == (3,)
+        idx, gates, counts, losses, stats = torch.ops.tmoe_b200.route_tokens(torch.empty(3, 7, 40), None, 2, 0, 10.0, 0.5)
+        assert idx.shape == gates.shape == (3, 7, 2) and idx.dtype == counts.dtype == torch.int32 and counts.shape == (40,) and losses.shape == (3,) and stats.shape == (3, 7, 2)
         assert torch.ops.tmoe_b200.expert_coefficients(idx, gates, torch.empty(40, 6)).shape == (3, 7, 6)
 
 

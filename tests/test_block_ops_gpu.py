@@ -354,10 +354,19 @@ def test_route_ties_signed_zeros_and_nan():
     s[2, ::2] = 1.0
     s[3, 6] = float("nan")
     s[3, 2] = 5.0
+    s[3, 9] = -float("nan")
     for dtype in (BF, F32):
         r = route_tokens(s.to(dtype).cuda(), 3)
-        assert r.idx.tolist() == [[0, 1, 2], [0, 1, 2], [0, 2, 4], [6, 2, 0]]
+        assert r.idx.tolist() == [[0, 1, 2], [0, 1, 2], [0, 2, 4], [6, 9, 2]]
         assert bool(torch.isnan(r.gates[3]).all()) and bool(torch.isnan(r.balance_loss)) and bool(torch.isfinite(r.gates[:3]).all())
+
+
+def test_route_orders_subnormal_scores():
+    for dtype, tiny in ((BF, 2.0 ** -130), (F32, 2.0 ** -140)):
+        s = torch.zeros(1, 16)
+        s[0, 5], s[0, 9], s[0, 11] = tiny, 2 * tiny, -tiny
+        r = route_tokens(s.to(dtype).cuda(), 16)
+        assert r.idx[0].tolist() == [9, 5] + [e for e in range(16) if e not in (5, 9, 11)] + [11]
 
 
 def test_route_saturated_cap():
