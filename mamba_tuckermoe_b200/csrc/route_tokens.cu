@@ -167,43 +167,48 @@ template <bool WIDE> struct Chunk<float, WIDE> {
   __device__ __forceinline__ f2 get(int j) const { return pair(v[2 * j], v[2 * j + 1]); }
 };
 
-// tanh of two values.  Up to 1 in magnitude by the Pade approximant x (945 + 105 x^2 + x^4) / (945 + 420 x^2 + 15 x^4) that Lambert's continued
-// fraction gives (6e-8 off at 1, less below), beyond that by 1 - 2 e / (1 + e) with e = exp(-2|x|), whose error shrinks with e.  NaN stays
-// NaN; the branch is the warp's, and scores seldom reach the cap.
-__device__ __forceinline__ f2 tanh2(f2 x) {
-  const f2 q = mul2(x, x);
-  float da, db, xa, xb;
-  split(fma2(q, fma2(q, both(15.f), both(420.f)), both(945.f)), da, db);
-  f2 t = mul2(mul2(x, fma2(q, add2(q, both(105.f)), both(945.f))), pair(fast_rcp(da), fast_rcp(db)));
-  split(x, xa, xb);
-  const bool fa = fabsf(xa) > 1.f, fb = fabsf(xb) > 1.f;
-  if (__any_sync(0xffffffffu, fa || fb)) {
-    float ta, tb;
-    split(t, ta, tb);
-    const float ea = fast_exp2(fabsf(xa) * (-2.f * kLog2e)), eb = fast_exp2(fabsf(xb) * (-2.f * kLog2e));
-    if (fa) ta = copysignf(1.f - 2.f * ea * fast_rcp(1.f + ea), xa);
-    if (fb) tb = copysignf(1.f - 2.f * eb * fast_rcp(1.f + eb), xb);
-    t = pair(ta, tb);
+// Capped, tempered logits l = scale * tanh(v * inv_cap) of N values and, for GRAD, their derivatives.  tanh up to 1 in magnitude is the Pade
+// approximant x (945 + 105 x^2 + x^4) / (945 + 420 x^2 + 15 x^4) that Lambert's continued fraction gives (6e-8 off at 1, less below) with
+// derivative 1 - t^2.  Beyond that, where 1 - t^2 cancels, both come from e = exp(-2|x|), and a score of -inf, which the cap would make a number
+// again, is put back to -inf.  That second part is skipped unless a lane of the warp needs it: scores seldom reach the cap.  NaN stays NaN.
+template <int N2, bool GRAD>
+__device__ __forceinline__ void cap_logits(const RouteArgs &a, f2 (&l)[N2], f2 (&d)[GRAD ? N2 : 1]) {
+  f2 x[N2];
+  bool far = false;
+#pragma unroll
+  for (int j = 0; j < N2; ++j) {
+    x[j] = mul2(l[j], both(a.inv_cap));
+    float xa, xb, da, db;
+    split(x[j], xa, xb);
+    far = far || fabsf(xa) > 1.f || fabsf(xb) > 1.f;
+    const f2 q = mul2(x[j], x[j]);
+    split(fma2(q, fma2(q, both(15.f), both(420.f)), both(945.f)), da, db);
+    const f2 t = mul2(mul2(x[j], fma2(q, add2(q, both(105.f)), both(945.f))), pair(fast_rcp(da), fast_rcp(db)));
+    l[j] = mul2(t, both(a.scale));
+    if (GRAD) d[j] = mul2(fma2(mul2(t, both(-1.f)), t, both(1.f)), both(a.scale * a.inv_cap));
   }
-  return t;
-}
-// 1 - tanh^2 at x, given t = tanh(x): from t up to 1, from e beyond, where 1 - t^2 would cancel
-__device__ __forceinline__ f2 sech2(f2 x, f2 t) {
-  f2 r = fma2(mul2(t, both(-1.f)), t, both(1.f));
-  float xa, xb;
-  split(x, xa, xb);
-  const bool fa = fabsf(xa) > 1.f, fb = fabsf(xb) > 1.f;
-  if (__any_sync(0xffffffffu, fa || fb)) {
-    float ra, rb;
-    split(r, ra, rb);
-    const float ea = fast_exp2(fabsf(xa) * (-2.f * kLog2e)), eb = fast_exp2(fabsf(xb) * (-2.f * kLog2e));
-    const float ia = fast_rcp(1.f + ea), ib = fast_rcp(1.f + eb);
-    if (fa) ra = 4.f * ea * ia * ia;
-    if (fb) rb = 4.f * eb * ib * ib;
-    r = pair(ra, rb);
+  if (!__any_sync(0xffffffffu, far)) return;
+#pragma unroll
+  for (int j = 0; j < N2; ++j) {
+    float v[2], lj[2], dj[2] = {0.f, 0.f};
+    split(x[j], v[0], v[1]);
+    split(l[j], lj[0], lj[1]);
+    if (GRAD) split(d[j], dj[0], dj[1]);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float e = fast_exp2(fabsf(v[h]) * (-2.f * kLog2e)), i = fast_rcp(1.f + e);
+      if (fabsf(v[h]) > 1.f) {
+        lj[h] = v[h] == -INFINITY ? -INFINITY : copysignf(fmaf(-2.f * e, i, 1.f), v[h]) * a.scale;
+        dj[h] = 4.f * e * i * i * (a.scale * a.inv_cap);
+      }
+    }
+    l[j] = pair(lj[0], lj[1]);
+    if (GRAD) d[j] = pair(dj[0], dj[1]);
   }
-  return r;
 }
+
+__device__ __forceinline__ float fast_log2(float x) { float r; asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+constexpr float kLn2 = 0.6931471805599453f;
 
 template <typename K> __device__ __forceinline__ void sort_two(K &a, K &b) {   // larger first
   const K hi = a > b ? a : b, lo = a > b ? b : a;
@@ -259,15 +264,23 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_const
   for (int x = 0; x < N / 2; ++x) acc[x] = both(0.f);
   float zsum = 0.f, nsum = 0.f;
   const int64_t step = (int64_t)gridDim.x * kRouteWarps * PER;
-  for (int64_t t0 = ((int64_t)blockIdx.x * kRouteWarps + warp) * PER; t0 < a.tokens; t0 += step) {
-    const int64_t t = t0 + grp;
+  int64_t t = ((int64_t)blockIdx.x * kRouteWarps + warp) * PER + grp;
+  Chunk<TS, WIDE> next[NC];                                   // one token ahead
+  auto fetch = [&](int64_t at) {
+    const bool want = at < a.tokens && (!a.mask || a.mask[at]);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) next[c].load((const TS *)a.scores + at * a.stride, (c * G + gl) * 8, a.E, want);
+  };
+  fetch(t);
+  for (; t - grp < a.tokens; t += step) {
     const bool here = t < a.tokens;
-    const bool want = here && (!a.mask || a.mask[t]);
     Chunk<TS, WIDE> s[NC];
     typename K::type key[NC][8];
 #pragma unroll
+    for (int c = 0; c < NC; ++c) s[c] = next[c];
+    fetch(t + step);
+#pragma unroll
     for (int c = 0; c < NC; ++c) {
-      s[c].load((const TS *)a.scores + t * a.stride, (c * G + gl) * 8, a.E, want);
       s[c].keys((c * G + gl) * 8, key[c]);
       sort_keys<DEPTH>(key[c]);
     }
@@ -294,34 +307,34 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_const
       }
     }
     const bool live = !K::empty(first);
-    float ta, tb;
-    split(a.rule == 1 ? mul2(tanh2(mul2(both(K::value(first)), both(a.inv_cap))), both(a.scale)) : both(K::value(first)), ta, tb);
-    const float top = live ? ta : 0.f;
+    // logits of the chosen, then of all; the largest is the first chosen one's
+    f2 lm[(SL + 1) / 2], none[1];
+#pragma unroll
+    for (int i = 0; i < (SL + 1) / 2; ++i)
+      lm[i] = pair(K::value(mine[2 * i]), 2 * i + 1 < SL ? K::value(mine[2 * i + 1 < SL ? 2 * i + 1 : 0]) : 0.f);
+    if (a.rule == 1) cap_logits<(SL + 1) / 2, false>(a, lm, none);
+    float la, lb;
+    split(lm[0], la, lb);
+    const float lead = __shfl_sync(0xffffffffu, la, lane - gl);
+    const float top = live ? lead : 0.f;
     f2 ex[N / 2], sum = both(0.f);
 #pragma unroll
+    for (int x = 0; x < N / 2; ++x) ex[x] = s[x / 4].get(x % 4);
+    if (a.rule == 1) cap_logits<N / 2, false>(a, ex, none);
+#pragma unroll
     for (int x = 0; x < N / 2; ++x) {
-      const f2 v = s[x / 4].get(x % 4);
-      f2 l = v;
-      if (a.rule == 1) l = mul2(tanh2(mul2(v, both(a.inv_cap))), both(a.scale));
-      float la, lb;
-      split(mul2(add2(l, both(-top)), both(kLog2e)), la, lb);   // (the difference first: exact for what matters, whatever the scores' size)
-      float ea = fast_exp2(la), eb = fast_exp2(lb);
-      if (a.rule == 1) {   // the cap makes -inf a number again
-        float va, vb;
-        split(v, va, vb);
-        ea = va == -INFINITY ? 0.f : ea;
-        eb = vb == -INFINITY ? 0.f : eb;
-      }
-      ex[x] = pair(ea, eb);
+      // (the difference first: exact for what matters, whatever the scores' size)
+      split(mul2(add2(ex[x], both(-top)), both(kLog2e)), la, lb);
+      ex[x] = pair(fast_exp2(la), fast_exp2(lb));
       sum = add2(sum, ex[x]);
     }
     const float den = group_sum<G>(sum2(sum));
-    const float inv = live ? 1.f / den : 0.f;
+    const float inv = live ? fast_rcp(den) : 0.f;
     if (live) {
 #pragma unroll
       for (int x = 0; x < N / 2; ++x) acc[x] = fma2(ex[x], both(inv), acc[x]);
       if (gl == 0) {
-        const float lse = top + logf(den);
+        const float lse = fmaf(fast_log2(den), kLn2, top);
         zsum = fmaf(lse, lse, zsum);
         nsum += 1.f;
         if (a.stats) reinterpret_cast<float2 *>(a.stats)[t] = make_float2(top, den);
@@ -330,27 +343,22 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_const
     float g[SL], total = 0.f;
 #pragma unroll
     for (int i = 0; i < SL; ++i) {
-      g[i] = 0.f;
-      if (i * G < a.k) {   // (uniform)
-        float va, vb;
-        split(a.rule == 1 ? mul2(tanh2(mul2(both(K::value(mine[i])), both(a.inv_cap))), both(a.scale)) : both(K::value(mine[i])), va, vb);
-        if (!K::empty(mine[i])) g[i] = fast_exp2((va - top) * kLog2e);
-        if (a.rule == 1) g[i] *= inv;
-        total += g[i];
-      }
+      split(lm[i / 2], la, lb);
+      g[i] = K::empty(mine[i]) ? 0.f : fast_exp2(((i & 1 ? lb : la) - top) * kLog2e) * (a.rule == 1 ? inv : 1.f);
+      total += g[i];
     }
     total = group_sum<G>(total);
-    if (a.rule == 1) total += 1e-6f;
-    const float over = live ? 1.f / total : 0.f;
+    const float over = live ? fast_rcp(a.rule == 1 ? total + 1e-6f : total) : 0.f;
     if (here) {
 #pragma unroll
       for (int i = 0; i < SL; ++i) {
         const int j = i * G + gl;
         if (j < a.k) {
           const bool full = !K::empty(mine[i]);
-          a.idx[t * a.k + j] = full ? K::col(mine[i]) : -1;
-          a.gates[t * a.k + j] = full ? g[i] * over : 0.f;
-          if (full) atomicAdd(&hist[K::col(mine[i])], 1);
+          const int col = K::col(mine[i]);
+          a.idx[t * a.k + j] = full ? col : -1;
+          a.gates[t * a.k + j] = g[i] * over;
+          if (full) atomicAdd(&hist[col], 1);
         }
       }
     }
@@ -488,81 +496,89 @@ __global__ void __launch_bounds__(kRouteThreads) route_backward_kernel(const __g
     A[x] = pair(col < a.E ? bal * (float)a.counts[col] : 0.f, col + 1 < a.E ? bal * (float)a.counts[col + 1] : 0.f);
   }
   const int64_t step = (int64_t)gridDim.x * kRouteWarps * PER;
-  for (int64_t t0 = ((int64_t)blockIdx.x * kRouteWarps + warp) * PER; t0 < a.tokens; t0 += step) {
-    const int64_t t = t0 + grp;
-    const bool here = t < a.tokens;
-    const bool want = here && (!a.mask || a.mask[t]);
+  int64_t t = ((int64_t)blockIdx.x * kRouteWarps + warp) * PER + grp;
+  struct Token {
     Chunk<TS, WIDE> s[NC];
+    float2 stat;
+    int col[SL];              // slots: lane j % G holds slot j
+    float g[SL], dg[SL];
+    bool live;                // a token that counts has a chosen expert in slot 0
+  };
+  auto fetch = [&](Token &n, int64_t at) {
+    const bool want = at < a.tokens && (!a.mask || a.mask[at]);
 #pragma unroll
-    for (int c = 0; c < NC; ++c) s[c].load((const TS *)a.scores + t * a.stride, (c * G + gl) * 8, a.E, want);
-    // slots: lane j % G holds slot j
-    int col[SL];
-    float val[SL], dg[SL], inner = 0.f, total = 0.f;
+    for (int c = 0; c < NC; ++c) n.s[c].load((const TS *)a.scores + at * a.stride, (c * G + gl) * 8, a.E, want);
+    n.live = false;
+    n.stat = make_float2(0.f, 1.f);
+    if (want) {
+      n.live = a.idx[at * a.k] >= 0;
+      n.stat = reinterpret_cast<const float2 *>(a.stats)[at];   // (not used unless live)
+    }
 #pragma unroll
     for (int i = 0; i < SL; ++i) {
       const int j = i * G + gl;
-      col[i] = -1; val[i] = dg[i] = 0.f;
+      n.col[i] = -1; n.g[i] = n.dg[i] = 0.f;
       if (a.d_gates && want && j < a.k) {
-        col[i] = a.idx[t * a.k + j];
-        if ((unsigned)col[i] >= (unsigned)a.E) col[i] = -1;
-        if (col[i] >= 0) {
-          val[i] = a.gates[t * a.k + j];
-          dg[i] = a.d_gates[t * a.k + j];
-          inner = fmaf(val[i], dg[i], inner);
-          total += val[i];
-        }
+        n.col[i] = a.idx[at * a.k + j];
+        n.g[i] = a.gates[at * a.k + j];
+        n.dg[i] = a.d_gates[at * a.k + j];
       }
     }
-    // a token that counts has a chosen expert in slot 0, and statistics
-    const bool live = want && a.idx[t * a.k] >= 0;
-    const float2 stat = live ? reinterpret_cast<const float2 *>(a.stats)[t] : make_float2(0.f, 1.f);
-    const float lse = stat.x + logf(stat.y), inv = 1.f / stat.y;
+  };
+  Token next;
+  fetch(next, t);
+  for (; t - grp < a.tokens; t += step) {
+    const bool here = t < a.tokens;
+    Token now = next;
+    fetch(next, t + step);                       // one token ahead
+    const float top = now.live ? now.stat.x : 0.f, den = now.live ? now.stat.y : 1.f;
+    const float lse = now.live ? fmaf(fast_log2(den), kLn2, top) : 0.f, inv = fast_rcp(den);
+    float inner = 0.f, total = 0.f;
+#pragma unroll
+    for (int i = 0; i < SL; ++i) {
+      const bool full = now.live && (unsigned)now.col[i] < (unsigned)a.E;   // (an empty slot's gradient may be anything)
+      now.col[i] = full ? now.col[i] : -1;
+      now.g[i] = full ? now.g[i] : 0.f;
+      now.dg[i] = full ? now.dg[i] : 0.f;
+      inner = fmaf(now.g[i], now.dg[i], inner);
+      total += now.g[i];
+    }
     f2 p[N / 2], th[N / 2], dot2 = both(0.f);
 #pragma unroll
+    for (int x = 0; x < N / 2; ++x) { p[x] = now.s[x / 4].get(x % 4); th[x] = both(1.f); }
+    if (a.rule == 1) cap_logits<N / 2, true>(a, p, th);
+#pragma unroll
     for (int x = 0; x < N / 2; ++x) {
-      const f2 v = s[x / 4].get(x % 4);
-      f2 l = v;
-      th[x] = both(1.f);
-      if (a.rule == 1) {
-        const f2 y = mul2(v, both(a.inv_cap)), t1 = tanh2(y);
-        th[x] = mul2(sech2(y, t1), both(a.scale * a.inv_cap));
-        l = mul2(t1, both(a.scale));
-      }
-      float la, lb, va, vb;
-      split(mul2(add2(l, both(-stat.x)), both(kLog2e)), la, lb);
-      split(v, va, vb);
-      p[x] = mul2(pair(va == -INFINITY ? 0.f : fast_exp2(la), vb == -INFINITY ? 0.f : fast_exp2(lb)), both(inv));
+      float la, lb;
+      split(mul2(add2(p[x], both(-top)), both(kLog2e)), la, lb);
+      p[x] = mul2(pair(fast_exp2(la), fast_exp2(lb)), both(inv));
       dot2 = fma2(p[x], A[x], dot2);
     }
-    const float dot = group_sum<G>(sum2(dot2));
-    float base = z2 * lse - dot;
+    float base = z2 * lse - group_sum<G>(sum2(dot2));
     if (a.d_gates) {
       inner = group_sum<G>(inner);
       if (a.rule == 1) base -= inner * (1.f - group_sum<G>(total));
 #pragma unroll
       for (int i = 0; i < SL; ++i)
-        if (col[i] >= 0) row[col[i]] = val[i] * (dg[i] - inner);
+        if (now.col[i] >= 0) row[now.col[i]] = now.g[i] * (now.dg[i] - inner);
       __syncwarp();
     }
     TS *dst = (TS *)a.d_scores + t * a.E;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int e0 = (c * G + gl) * 8;
-      f2 d[4];
       float4 r0 = make_float4(0.f, 0.f, 0.f, 0.f), r1 = r0;
       if (a.d_gates) { r0 = *reinterpret_cast<const float4 *>(row + e0); r1 = *reinterpret_cast<const float4 *>(row + e0 + 4); }
-      d[0] = pair(r0.x, r0.y); d[1] = pair(r0.z, r0.w); d[2] = pair(r1.x, r1.y); d[3] = pair(r1.z, r1.w);
+      const f2 chosen[4] = {pair(r0.x, r0.y), pair(r0.z, r0.w), pair(r1.x, r1.y), pair(r1.z, r1.w)};
       float f[8];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int x = c * 4 + j;
-        d[j] = mul2(fma2(p[x], add2(A[x], both(base)), d[j]), th[x]);
-        split(d[j], f[2 * j], f[2 * j + 1]);
-        // an expert that is off, a token that does not count: no gradient (sech^2 of -inf is 0 by itself; rule 0 needs the test)
-        float va, vb;
-        split(s[c].get(j), va, vb);
-        if (va == -INFINITY) f[2 * j] = 0.f;
-        if (vb == -INFINITY) f[2 * j + 1] = 0.f;
+        split(mul2(fma2(p[x], add2(A[x], both(base)), chosen[j]), th[x]), f[2 * j], f[2 * j + 1]);
+      }
+      if (!now.live) {      // (whatever the upstream gradients hold)
+#pragma unroll
+        for (int q = 0; q < 8; ++q) f[q] = 0.f;
       }
       if (here) {
         if (WIDE) {
@@ -586,7 +602,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_backward_kernel(const __g
       __syncwarp();
 #pragma unroll
       for (int i = 0; i < SL; ++i)
-        if (col[i] >= 0) row[col[i]] = 0.f;
+        if (now.col[i] >= 0) row[now.col[i]] = 0.f;
       __syncwarp();
     }
   }
@@ -599,7 +615,7 @@ int lanes_per_token(int E) {
 }
 int route_blocks(int64_t tokens, int E, int sms) {
   const int64_t per = kRouteWarps * (32 / lanes_per_token(E));
-  const int64_t want = (tokens + per - 1) / per, cap = (int64_t)sms * 3;
+  const int64_t want = (tokens + per - 1) / per, cap = (int64_t)sms * 4;
   return (int)(want < cap ? want : cap);
 }
 
