@@ -6,17 +6,20 @@
 //
 // A slot whose index lies outside 0 .. E-1 is empty: it adds nothing and its d_gates is 0.
 //
-// d_U is a scatter of T * k rows onto E; float atomics would add them in another order on every run.  Here each group of lanes
-// keeps a table [E, columns] of its own in shared memory and adds its slots to it in order; a block adds its groups' tables in
-// order and writes one partial table, coef_reduce_kernel adds the blocks' tables in order.
+// d_U is a scatter of T * k rows onto E; float atomics would add them in another order on every run.  Here each group of lanes keeps a
+// table [E, columns] of its own in shared memory and adds its tokens' slots to it in order; a block adds its groups' tables in order
+// and writes one partial table, coef_reduce_kernel adds the blocks' tables in order.
 #include "common.cuh"
 #include "kernels.h"
+#include "ptx.cuh"
 
 namespace tmoe {
 namespace {
 
 constexpr int kCoefMaxExperts = 16384;
 constexpr int kCoefSmem = 160 * 1024;    // shared memory for the tables of one block
+constexpr int kDuThreads = 640;          // 20 warps of up to 96 registers
+constexpr int kAhead = 8;                // rounds of slots whose operands are in flight
 
 struct CoefArgs {
   const int32_t *idx;     // [T, k]
@@ -30,22 +33,75 @@ struct CoefArgs {
   float *partial;         // [blocks, E, r1]
 };
 
-template <typename TU>
-__global__ void __launch_bounds__(256) coef_kernel(const __grid_constant__ CoefArgs a) {
-  const int64_t n = a.T * a.r1;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    const int64_t t = i / a.r1;
-    const int col = (int)(i - t * a.r1);
-    float s = 0.f;
-    for (int j = 0; j < a.k; ++j) {
-      const int e = a.idx[t * a.k + j];
-      if ((unsigned)e < (unsigned)a.E) s = fmaf(a.gates[t * a.k + j], to_f32(((const TU *)a.u)[(int64_t)e * a.r1 + col]), s);
+// C consecutive values of a U_expert row or an fp32 row (C = 4: one 8- or 16-byte load)
+template <int C> __device__ __forceinline__ void load_cols(const float *p, float (&f)[C]) {
+  if constexpr (C == 4) {
+    const float4 v = __ldg(reinterpret_cast<const float4 *>(p));
+    f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+  } else {
+    f[0] = __ldg(p);
+  }
+}
+template <int C> __device__ __forceinline__ void load_cols(const bf16 *p, float (&f)[C]) {
+  if constexpr (C == 4) {
+    const uint2 v = __ldg(reinterpret_cast<const uint2 *>(p));
+    f[0] = __uint_as_float(v.x << 16); f[1] = __uint_as_float(v.x & 0xffff0000u);
+    f[2] = __uint_as_float(v.y << 16); f[3] = __uint_as_float(v.y & 0xffff0000u);
+  } else {
+    f[0] = to_f32(*p);
+  }
+}
+// up to 4 slots of a token (KV = 4: one 16-byte load each)
+template <int KV> struct SlotPack {
+  int e[KV];
+  float g[KV];
+  __device__ __forceinline__ void load(const CoefArgs &a, int64_t at) {
+    if constexpr (KV == 4) {
+      const int4 i = __ldg(reinterpret_cast<const int4 *>(a.idx + at));
+      const float4 f = __ldg(reinterpret_cast<const float4 *>(a.gates + at));
+      e[0] = i.x; e[1] = i.y; e[2] = i.z; e[3] = i.w;
+      g[0] = f.x; g[1] = f.y; g[2] = f.z; g[3] = f.w;
+    } else if constexpr (KV == 2) {
+      const int2 i = __ldg(reinterpret_cast<const int2 *>(a.idx + at));
+      const float2 f = __ldg(reinterpret_cast<const float2 *>(a.gates + at));
+      e[0] = i.x; e[1] = i.y; g[0] = f.x; g[1] = f.y;
+    } else {
+      e[0] = __ldg(a.idx + at); g[0] = __ldg(a.gates + at);
     }
-    a.c[i] = s;
+  }
+};
+
+// One thread makes C neighbouring coefficients of a token; the U_expert table comes from L1.
+template <typename TU, int C, int KV>
+__global__ void __launch_bounds__(256) coef_kernel(const __grid_constant__ CoefArgs a) {
+  const int per = a.r1 / C;
+  const int64_t n = a.T * per;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t t = i / per;
+    const int col = (int)(i - t * per) * C;
+    float s[C];
+#pragma unroll
+    for (int q = 0; q < C; ++q) s[q] = 0.f;
+    for (int j = 0; j < a.k; j += KV) {
+      SlotPack<KV> p;
+      p.load(a, t * a.k + j);
+#pragma unroll
+      for (int v = 0; v < KV; ++v) {
+        if ((unsigned)p.e[v] < (unsigned)a.E) {
+          float u[C];
+          load_cols<C>((const TU *)a.u + (int64_t)p.e[v] * a.r1 + col, u);
+#pragma unroll
+          for (int q = 0; q < C; ++q) s[q] = fmaf(p.g[v], u[q], s[q]);
+        }
+      }
+    }
+    if constexpr (C == 4) *reinterpret_cast<float4 *>(a.c + t * a.r1 + col) = make_float4(s[0], s[1], s[2], s[3]);
+    else a.c[t * a.r1 + col] = s[0];
   }
 }
 
-template <typename TU>
+// One thread per slot.
+template <typename TU, int C>
 __global__ void __launch_bounds__(256) coef_d_gates_kernel(const __grid_constant__ CoefArgs a) {
   const int64_t n = a.T * a.k;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
@@ -54,36 +110,86 @@ __global__ void __launch_bounds__(256) coef_d_gates_kernel(const __grid_constant
     if ((unsigned)e < (unsigned)a.E) {
       const float *d = a.d_c + (i / a.k) * a.r1;
       const TU *u = (const TU *)a.u + (int64_t)e * a.r1;
-      for (int q = 0; q < a.r1; ++q) s = fmaf(to_f32(u[q]), d[q], s);
+#pragma unroll 2
+      for (int q = 0; q < a.r1; q += C) {
+        float x[C], y[C];
+        load_cols<C>(u + q, x);
+        load_cols<C>(d + q, y);
+#pragma unroll
+        for (int v = 0; v < C; ++v) s = fmaf(x[v], y[v], s);
+      }
     }
     a.d_gates[i] = s;
   }
 }
 
-// blockDim = groups * cols; blockIdx.y picks the columns.
-__global__ void __launch_bounds__(1024) coef_d_u_kernel(const __grid_constant__ CoefArgs a, int cols) {
-  extern __shared__ float tab[];   // [groups][E * cols]
-  const int groups = blockDim.x / cols, grp = threadIdx.x / cols, col = threadIdx.x - grp * cols;
-  const int c0 = blockIdx.y * cols, width = a.E * cols;
+// A group of S * L lanes (a power of two up to 32) takes S slots of a token at once, L columns each, with a private table.  The experts of a
+// token usually differ, so the S slots touch different rows of it; where an expert is given twice the lanes take turns.  The next slots'
+// operands are loaded while these are added.  blockIdx.y picks the columns; threads beyond the last group only keep their warp whole.
+template <int L>
+__global__ void __launch_bounds__(kDuThreads) coef_d_u_kernel(const __grid_constant__ CoefArgs a, int S, int groups) {
+  extern __shared__ __align__(16) float tab[];   // [groups][E * L]
+  const int lanes = S * L, grp = threadIdx.x / lanes, in = threadIdx.x - grp * lanes, lane = threadIdx.x & 31;
+  const int s = in / L, col = in - s * L, c = blockIdx.y * L + col, width = a.E * L;
+  ptx::griddep_launch_dependents();
   for (int i = threadIdx.x; i < groups * width; i += blockDim.x) tab[i] = 0.f;
-  __syncthreads();
-  if (c0 + col < a.r1) {
-    float *mine = tab + grp * width + col;
-    const int64_t lo = a.T * blockIdx.x / gridDim.x, hi = a.T * (blockIdx.x + 1) / gridDim.x;
-    for (int64_t t = lo + grp; t < hi; t += groups) {
-      const float d = a.d_c[t * a.r1 + c0 + col];
-      for (int j = 0; j < a.k; ++j) {
-        const int e = a.idx[t * a.k + j];
-        if ((unsigned)e < (unsigned)a.E) mine[e * cols] = fmaf(a.gates[t * a.k + j], d, mine[e * cols]);
+  // the lanes of this group that hold the same column of the other slots before this one
+  uint32_t before = 0;
+  for (int q = 0; q < s; ++q) before |= 1u << ((lane & ~(lanes - 1)) + q * L + col);
+  const int64_t lo = a.T * blockIdx.x / gridDim.x, hi = a.T * (blockIdx.x + 1) / gridDim.x;
+  // every lane of the block walks the same number of rounds: the turns need whole warps (rounds beyond the last are empty)
+  const int rounds = (int)((hi - lo + groups - 1) / groups) * ((a.k + S - 1) / S);
+  int64_t t = grp < groups ? lo + grp : hi;
+  int64_t slot = t * a.k, at = t * a.r1 + c;
+  int j = s;
+  int e_next[kAhead], e[kAhead];
+  float g_next[kAhead], d_next[kAhead], g[kAhead], d[kAhead];
+  auto fetch = [&]() {
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q) {
+      e_next[q] = -1;
+      if (t < hi && j < a.k && c < a.r1) {
+        e_next[q] = __ldg(a.idx + slot + j);
+        g_next[q] = __ldg(a.gates + slot + j);
+        d_next[q] = __ldg(a.d_c + at);
       }
+      j += S;
+      if (j - s >= a.k) { j = s; t += groups; slot += (int64_t)groups * a.k; at += (int64_t)groups * a.r1; }
+    }
+  };
+  fetch();
+  __syncthreads();
+  float *mine = tab + (grp < groups ? grp * width + col : 0);
+  for (int r = 0; r < rounds; r += kAhead) {
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q) { e[q] = e_next[q]; g[q] = g_next[q]; d[q] = d_next[q]; }
+    if (r + kAhead < rounds) fetch();
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q) {
+      const bool have = (unsigned)e[q] < (unsigned)a.E;
+      bool twice = false;
+      for (int o = L; o < lanes; o += L) {
+        const int other = __shfl_xor_sync(0xffffffffu, e[q], o);   // by every lane, whatever it has found
+        twice |= other == e[q];
+      }
+      if (!__any_sync(0xffffffffu, have && twice)) {
+        if (have) mine[e[q] * L] = fmaf(g[q], d[q], mine[e[q] * L]);
+      } else {
+        const int turn = __popc(__match_any_sync(0xffffffffu, have ? e[q] : -1 - lane) & before);
+        for (int w = 0; w < S; ++w) {
+          if (have && turn == w) mine[e[q] * L] = fmaf(g[q], d[q], mine[e[q] * L]);
+          __syncwarp();
+        }
+      }
+      __syncwarp();   // the group's other lanes may hold this row next
     }
   }
   __syncthreads();
   for (int i = threadIdx.x; i < width; i += blockDim.x) {
-    float s = 0.f;
-    for (int g = 0; g < groups; ++g) s += tab[g * width + i];
-    const int e = i / cols, q = i - e * cols;
-    if (c0 + q < a.r1) a.partial[((int64_t)blockIdx.x * a.E + e) * a.r1 + c0 + q] = s;
+    float v = 0.f;
+    for (int q = 0; q < groups; ++q) v += tab[q * width + i];
+    const int x = i / L, q = i - x * L;
+    if (blockIdx.y * L + q < a.r1) a.partial[((int64_t)blockIdx.x * a.E + x) * a.r1 + blockIdx.y * L + q] = v;
   }
 }
 
@@ -91,9 +197,12 @@ template <typename TU>
 __global__ void __launch_bounds__(256) coef_reduce_kernel(const float *__restrict__ partial, int blocks, int n, TU *__restrict__ d_u) {
   __shared__ float part[8][33];
   const int col = blockIdx.x * 32 + (threadIdx.x & 31), lane = threadIdx.x & 31, row = threadIdx.x >> 5;
+  ptx::griddep_wait();
   float s = 0.f;
-  if (col < n)
+  if (col < n) {
+#pragma unroll 4
     for (int b = row; b < blocks; b += 8) s += partial[(int64_t)b * n + col];
+  }
   part[row][lane] = s;
   __syncthreads();
   if (row == 0 && col < n) {
@@ -124,21 +233,52 @@ CoefArgs coef_args(const tmoe_expert_coef_t &p) {
   return a;
 }
 
-// Columns of one block and its lane groups: as many private tables as fit
-struct DuShape { int cols, groups, parts; };
-DuShape du_shape(int E, int r1) {
+// Columns of a block (L), slots taken at once (S), groups with a table each, blocks over the tokens.  Tables of at most 32 KB leave room for
+// several groups; a group wants some rounds of work for the table it clears and folds.
+struct DuShape { int L, S, parts, groups, blocks; };
+DuShape du_shape(int64_t T, int E, int k, int r1, int sms) {
   DuShape s;
-  s.cols = 1;
-  while (s.cols < 32 && s.cols < r1 && (int64_t)E * s.cols * 2 * 4 <= 32 * 1024) s.cols *= 2;
-  s.parts = (r1 + s.cols - 1) / s.cols;
-  s.groups = (int)(kCoefSmem / ((int64_t)E * s.cols * 4));
-  if (s.groups > 512 / s.cols) s.groups = 512 / s.cols;
+  s.L = 1;
+  while (s.L < 32 && s.L < r1 && (int64_t)E * s.L * 2 * 4 <= 32 * 1024) s.L *= 2;
+  s.parts = (r1 + s.L - 1) / s.L;
+  s.S = 1;
+  while (s.S < k && s.S * 2 * s.L <= 32) s.S *= 2;
+  const int most = (int)(kCoefSmem / ((int64_t)E * s.L * 4)), lanes = s.S * s.L;
+  const int64_t cap = (sms + s.parts - 1) / s.parts, want = (T + 31) / 32;
+  s.blocks = (int)(want < cap ? want : cap);
+  const int64_t each = (T + s.blocks - 1) / s.blocks, rounds = 8 / ((k + s.S - 1) / s.S) > 0 ? 8 / ((k + s.S - 1) / s.S) : 1;
+  s.groups = (int)((each + rounds - 1) / rounds);
+  if (s.groups > most) s.groups = most;
+  if (s.groups > kDuThreads / lanes) s.groups = kDuThreads / lanes;
   return s;
 }
-int du_blocks(int64_t T, int E, int r1, int sms) {
-  const DuShape s = du_shape(E, r1);
-  const int64_t want = (T + s.groups * 4 - 1) / (s.groups * 4), cap = (sms + s.parts - 1) / s.parts;
-  return (int)(want < cap ? want : cap);
+
+template <int L>
+int launch_d_u(const CoefArgs &a, const DuShape &s, cudaStream_t st) {
+  static std::atomic<uint64_t> opted{0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return TMOE_ERR_CUDA;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(opted.load(std::memory_order_relaxed) & bit)) {
+    if (cudaFuncSetAttribute(coef_d_u_kernel<L>, cudaFuncAttributeMaxDynamicSharedMemorySize, kCoefSmem) != cudaSuccess) return TMOE_ERR_CUDA;
+    opted.fetch_or(bit, std::memory_order_relaxed);
+  }
+  const int threads = (s.groups * s.S * s.L + 31) / 32 * 32;
+  coef_d_u_kernel<L><<<dim3(s.blocks, s.parts), threads, (size_t)s.groups * a.E * s.L * 4, st>>>(a, s.S, s.groups);
+  count_launch();
+  return launch_status();
+}
+
+// wide: rows of U_expert, c and d_c are whole 4-column pieces
+bool cols_by_4(const CoefArgs &a, int size, const void *rows) {
+  return a.r1 % 4 == 0 && !(reinterpret_cast<uintptr_t>(a.u) & (4 * size - 1)) && !(reinterpret_cast<uintptr_t>(rows) & 15);
+}
+template <typename TU, int C>
+void launch_coef(const CoefArgs &a, int blocks, cudaStream_t st) {
+  const uintptr_t both = reinterpret_cast<uintptr_t>(a.idx) | reinterpret_cast<uintptr_t>(a.gates);
+  if (a.k % 4 == 0 && !(both & 15)) coef_kernel<TU, C, 4><<<blocks, 256, 0, st>>>(a);
+  else if (a.k % 2 == 0 && !(both & 7)) coef_kernel<TU, C, 2><<<blocks, 256, 0, st>>>(a);
+  else coef_kernel<TU, C, 1><<<blocks, 256, 0, st>>>(a);
 }
 
 }  // namespace
@@ -158,10 +298,12 @@ int tmoe_expert_coef(const tmoe_expert_coef_t *p, float *c, void *stream) {
   if (sms <= 0) return TMOE_ERR_CUDA;
   CoefArgs a = coef_args(*p);
   a.c = c;
-  const int64_t want = (a.T * a.r1 + 255) / 256, cap = (int64_t)sms * 16;
+  const bool four = cols_by_4(a, p->dtype == TMOE_F32 ? 4 : 2, c);
+  const int64_t want = (a.T * (a.r1 / (four ? 4 : 1)) + 255) / 256, cap = (int64_t)sms * 16;
   const int blocks = (int)(want < cap ? want : cap);
-  if (p->dtype == TMOE_F32) coef_kernel<float><<<blocks, 256, 0, (cudaStream_t)stream>>>(a);
-  else coef_kernel<bf16><<<blocks, 256, 0, (cudaStream_t)stream>>>(a);
+  cudaStream_t st = (cudaStream_t)stream;
+  if (p->dtype == TMOE_F32) four ? launch_coef<float, 4>(a, blocks, st) : launch_coef<float, 1>(a, blocks, st);
+  else four ? launch_coef<bf16, 4>(a, blocks, st) : launch_coef<bf16, 1>(a, blocks, st);
   count_launch();
   return launch_status();
 }
@@ -170,7 +312,7 @@ int64_t tmoe_expert_coef_workspace_bytes(const tmoe_expert_coef_t *p) {
   int rc = check_coef(p);
   if (rc) return rc;
   // sized for up to 160 SMs, whatever device the sizing query runs on
-  return p->tokens ? (int64_t)du_blocks(p->tokens, p->n_experts, p->r1, 160) * p->n_experts * p->r1 * 4 : 0;
+  return p->tokens ? (int64_t)du_shape(p->tokens, p->n_experts, p->top_k, p->r1, 160).blocks * p->n_experts * p->r1 * 4 : 0;
 }
 
 int tmoe_expert_coef_backward(const tmoe_expert_coef_t *p, const float *d_c, float *d_gates, void *d_U_expert, void *workspace,
@@ -192,27 +334,32 @@ int tmoe_expert_coef_backward(const tmoe_expert_coef_t *p, const float *d_c, flo
   if (d_gates) {
     const int64_t want = (a.T * a.k + 255) / 256, cap = (int64_t)sms * 16;
     const int blocks = (int)(want < cap ? want : cap);
-    if (p->dtype == TMOE_F32) coef_d_gates_kernel<float><<<blocks, 256, 0, st>>>(a);
-    else coef_d_gates_kernel<bf16><<<blocks, 256, 0, st>>>(a);
+    const bool four = cols_by_4(a, size, d_c);
+    if (p->dtype == TMOE_F32) four ? coef_d_gates_kernel<float, 4><<<blocks, 256, 0, st>>>(a) : coef_d_gates_kernel<float, 1><<<blocks, 256, 0, st>>>(a);
+    else four ? coef_d_gates_kernel<bf16, 4><<<blocks, 256, 0, st>>>(a) : coef_d_gates_kernel<bf16, 1><<<blocks, 256, 0, st>>>(a);
     count_launch();
     if ((rc = launch_status())) return rc;
   }
   if (d_U_expert) {
-    const DuShape s = du_shape(a.E, a.r1);
-    const int blocks = du_blocks(a.T, a.E, a.r1, sms < 160 ? sms : 160), n = a.E * a.r1;
+    const DuShape s = du_shape(a.T, a.E, a.k, a.r1, sms < 160 ? sms : 160);
+    const int n = a.E * a.r1;
     if (!workspace) return TMOE_ERR_NULL;
     if (reinterpret_cast<uintptr_t>(workspace) & 15) return TMOE_ERR_ALIGN;
-    if (workspace_bytes < (int64_t)blocks * n * 4) return TMOE_ERR_WORKSPACE;
+    if (workspace_bytes < (int64_t)s.blocks * n * 4) return TMOE_ERR_WORKSPACE;
     a.partial = reinterpret_cast<float *>(workspace);
-    const int smem = s.groups * a.E * s.cols * 4;
-    if (cudaFuncSetAttribute(coef_d_u_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kCoefSmem) != cudaSuccess) return TMOE_ERR_CUDA;
-    coef_d_u_kernel<<<dim3(blocks, s.parts), s.groups * s.cols, smem, st>>>(a, s.cols);
+    switch (s.L) {
+      case 1: rc = launch_d_u<1>(a, s, st); break;
+      case 2: rc = launch_d_u<2>(a, s, st); break;
+      case 4: rc = launch_d_u<4>(a, s, st); break;
+      case 8: rc = launch_d_u<8>(a, s, st); break;
+      case 16: rc = launch_d_u<16>(a, s, st); break;
+      default: rc = launch_d_u<32>(a, s, st); break;
+    }
+    if (rc) return rc;
+    const dim3 grid((unsigned)((n + 31) / 32)), block(256);
+    rc = p->dtype == TMOE_F32 ? cuda_ok(launch_pdl(coef_reduce_kernel<float>, grid, block, 0, st, a.partial, s.blocks, n, (float *)d_U_expert))
+                              : cuda_ok(launch_pdl(coef_reduce_kernel<bf16>, grid, block, 0, st, a.partial, s.blocks, n, (bf16 *)d_U_expert));
     count_launch();
-    if ((rc = launch_status())) return rc;
-    if (p->dtype == TMOE_F32) coef_reduce_kernel<float><<<(n + 31) / 32, 256, 0, st>>>(a.partial, blocks, n, (float *)d_U_expert);
-    else coef_reduce_kernel<bf16><<<(n + 31) / 32, 256, 0, st>>>(a.partial, blocks, n, (bf16 *)d_U_expert);
-    count_launch();
-    rc = launch_status();
   }
   return rc;
 }
