@@ -279,7 +279,7 @@ int tmoe_route_tokens_backward(const tmoe_route_t *p, const int32_t *idx, const 
  * that tmoe_in_core takes.  A slot whose index lies outside 0 .. n_experts-1 is empty. */
 typedef struct tmoe_expert_coef {
   int64_t tokens;          /* 0 .. 2^30 */
-  int32_t n_experts;       /* 1 .. 16384 (TMOE_ERR_UNSUPPORTED above) */
+  int32_t n_experts;       /* 1 .. 8192 (TMOE_ERR_UNSUPPORTED above) */
   int32_t top_k;           /* 1 .. TMOE_MAX_TOPK */
   int32_t r1;              /* 1 .. TMOE_MAX_R1 */
   int32_t dtype;           /* of U_expert */

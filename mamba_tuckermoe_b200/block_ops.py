@@ -490,7 +490,7 @@ def expert_coefficients(idx: torch.Tensor, gates: torch.Tensor, U_expert: torch.
 
     ``idx`` int32 and ``gates`` float32 ``(..., top_k)`` as ``route_tokens`` or ``forward_with_routing`` return them; a slot whose index
     lies outside ``0 .. E-1`` (an empty slot's is -1) adds nothing.  The same expert may appear in several slots of a token.
-    ``U_expert`` ``(E, r1)``, E up to 16384, r1 up to 64, ``top_k`` up to 16."""
+    ``U_expert`` ``(E, r1)``, E up to 8192, r1 up to 64, ``top_k`` up to 16."""
     if _is_compiling():
         return torch.ops.tmoe_b200.expert_coefficients(idx, gates, U_expert)
     if torch.is_grad_enabled() and (gates.requires_grad or U_expert.requires_grad):

@@ -9,6 +9,7 @@
 // d_U is a scatter of T * k rows onto E; float atomics would add them in another order on every run.  Here each group of lanes keeps a
 // table [E, columns] of its own in shared memory and adds its tokens' slots to it in order; a block adds its groups' tables in order
 // and writes one partial table, coef_reduce_kernel adds the blocks' tables in order.
+#include "column_sum.cuh"
 #include "common.cuh"
 #include "kernels.h"
 #include "ptx.cuh"
@@ -16,10 +17,10 @@
 namespace tmoe {
 namespace {
 
-constexpr int kCoefMaxExperts = 16384;
-constexpr int kCoefSmem = 160 * 1024;    // shared memory for the tables of one block
+constexpr int kCoefMaxExperts = 8192;    // a table of 4 columns: 128 KB
+constexpr int kCoefSmem = 192 * 1024;    // shared memory for the tables of one block
 constexpr int kDuThreads = 640;          // 20 warps of up to 96 registers
-constexpr int kAhead = 8;                // rounds of slots whose operands are in flight
+constexpr int kAhead = 4;                // rounds of slots whose operands are in flight
 
 struct CoefArgs {
   const int32_t *idx;     // [T, k]
@@ -100,66 +101,97 @@ __global__ void __launch_bounds__(256) coef_kernel(const __grid_constant__ CoefA
   }
 }
 
-// One thread per slot.
-template <typename TU, int C>
+// One thread makes KV neighbouring slots of a token.
+template <typename TU, int C, int KV>
 __global__ void __launch_bounds__(256) coef_d_gates_kernel(const __grid_constant__ CoefArgs a) {
-  const int64_t n = a.T * a.k;
+  ptx::griddep_launch_dependents();
+  const int per = a.k / KV;
+  const int64_t n = a.T * per;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    const int e = a.idx[i];
-    float s = 0.f;
-    if ((unsigned)e < (unsigned)a.E) {
-      const float *d = a.d_c + (i / a.k) * a.r1;
-      const TU *u = (const TU *)a.u + (int64_t)e * a.r1;
-#pragma unroll 2
-      for (int q = 0; q < a.r1; q += C) {
-        float x[C], y[C];
-        load_cols<C>(u + q, x);
-        load_cols<C>(d + q, y);
+    const int64_t t = i / per, at = i * KV;
+    SlotPack<KV> p;
+    p.load(a, at);
+    float s[KV];
 #pragma unroll
-        for (int v = 0; v < C; ++v) s = fmaf(x[v], y[v], s);
+    for (int v = 0; v < KV; ++v) {
+      s[v] = 0.f;
+      if ((unsigned)p.e[v] >= (unsigned)a.E) p.e[v] = -1;
+    }
+    for (int q = 0; q < a.r1; q += C) {
+      float d[C];
+      load_cols<C>(a.d_c + t * a.r1 + q, d);
+#pragma unroll
+      for (int v = 0; v < KV; ++v) {
+        if (p.e[v] >= 0) {
+          float u[C];
+          load_cols<C>((const TU *)a.u + (int64_t)p.e[v] * a.r1 + q, u);
+#pragma unroll
+          for (int x = 0; x < C; ++x) s[v] = fmaf(u[x], d[x], s[v]);
+        }
       }
     }
-    a.d_gates[i] = s;
+    if constexpr (KV == 4) *reinterpret_cast<float4 *>(a.d_gates + at) = make_float4(s[0], s[1], s[2], s[3]);
+    else if constexpr (KV == 2) *reinterpret_cast<float2 *>(a.d_gates + at) = make_float2(s[0], s[1]);
+    else a.d_gates[at] = s[0];
   }
 }
 
-// A group of S * L lanes (a power of two up to 32) takes S slots of a token at once, L columns each, with a private table.  The experts of a
-// token usually differ, so the S slots touch different rows of it; where an expert is given twice the lanes take turns.  The next slots'
-// operands are loaded while these are added.  blockIdx.y picks the columns; threads beyond the last group only keep their warp whole.
+// A group of S * L lanes (a power of two up to 32) takes S slots of a token at once, 4 columns a lane, with a private table.  The experts of
+// a token usually differ, so the S slots touch different rows of it; where an expert is given twice the lanes take turns.  The operands of
+// kAhead rounds are in flight while the ones before are added.  blockIdx.y picks the columns; threads beyond the last group only keep
+// their warp whole.
 template <int L>
-__global__ void __launch_bounds__(kDuThreads) coef_d_u_kernel(const __grid_constant__ CoefArgs a, int S, int groups) {
-  extern __shared__ __align__(16) float tab[];   // [groups][E * L]
+__global__ void __launch_bounds__(kDuThreads) coef_d_u_kernel(const __grid_constant__ CoefArgs a, int S, int groups, int wide) {
+  extern __shared__ __align__(16) float4 tab[];   // [groups][E * L]
   const int lanes = S * L, grp = threadIdx.x / lanes, in = threadIdx.x - grp * lanes, lane = threadIdx.x & 31;
-  const int s = in / L, col = in - s * L, c = blockIdx.y * L + col, width = a.E * L;
+  const int s = in / L, col = in - s * L, c = (blockIdx.y * L + col) * 4, width = a.E * L;
   ptx::griddep_launch_dependents();
-  for (int i = threadIdx.x; i < groups * width; i += blockDim.x) tab[i] = 0.f;
-  // the lanes of this group that hold the same column of the other slots before this one
+  for (int i = threadIdx.x; i < groups * width; i += blockDim.x) tab[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  // the lanes of this group that hold the same columns of the slots before this one
   uint32_t before = 0;
   for (int q = 0; q < s; ++q) before |= 1u << ((lane & ~(lanes - 1)) + q * L + col);
   const int64_t lo = a.T * blockIdx.x / gridDim.x, hi = a.T * (blockIdx.x + 1) / gridDim.x;
   // every lane of the block walks the same number of rounds: the turns need whole warps (rounds beyond the last are empty)
   const int rounds = (int)((hi - lo + groups - 1) / groups) * ((a.k + S - 1) / S);
-  int64_t t = grp < groups ? lo + grp : hi;
-  int64_t slot = t * a.k, at = t * a.r1 + c;
+  int left = grp < groups && c < a.r1 ? (int)((hi - lo - grp + groups - 1) / groups) : 0;   // tokens of this group
   int j = s;
+  const int64_t t0 = lo + (grp < groups ? grp : 0);
+  const int32_t *idx = a.idx + t0 * a.k;
+  const float *gates = a.gates + t0 * a.k, *d_c = a.d_c + t0 * a.r1 + c;
+  const int64_t k_step = (int64_t)groups * a.k, d_step = (int64_t)groups * a.r1;
   int e_next[kAhead], e[kAhead];
-  float g_next[kAhead], d_next[kAhead], g[kAhead], d[kAhead];
+  float g_next[kAhead], g[kAhead];
+  float4 d_next[kAhead], d[kAhead];
   auto fetch = [&]() {
 #pragma unroll
     for (int q = 0; q < kAhead; ++q) {
       e_next[q] = -1;
-      if (t < hi && j < a.k && c < a.r1) {
-        e_next[q] = __ldg(a.idx + slot + j);
-        g_next[q] = __ldg(a.gates + slot + j);
-        d_next[q] = __ldg(a.d_c + at);
+      g_next[q] = 0.f;
+      d_next[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (left > 0 && j < a.k) {
+        e_next[q] = __ldg(idx + j);
+        g_next[q] = __ldg(gates + j);
+        if (wide) {
+          d_next[q] = __ldg(reinterpret_cast<const float4 *>(d_c));
+        } else {
+          d_next[q].x = __ldg(d_c);
+          if (c + 1 < a.r1) d_next[q].y = __ldg(d_c + 1);
+          if (c + 2 < a.r1) d_next[q].z = __ldg(d_c + 2);
+          if (c + 3 < a.r1) d_next[q].w = __ldg(d_c + 3);
+        }
       }
       j += S;
-      if (j - s >= a.k) { j = s; t += groups; slot += (int64_t)groups * a.k; at += (int64_t)groups * a.r1; }
+      if (j - s >= a.k) { j = s; --left; idx += k_step; gates += k_step; d_c += d_step; }
     }
   };
   fetch();
   __syncthreads();
-  float *mine = tab + (grp < groups ? grp * width + col : 0);
+  float4 *mine = tab + (grp < groups ? grp * width + col : 0);
+  auto add = [&](int row, float w, const float4 &x) {
+    float4 v = mine[row * L];
+    v.x = fmaf(w, x.x, v.x); v.y = fmaf(w, x.y, v.y); v.z = fmaf(w, x.z, v.z); v.w = fmaf(w, x.w, v.w);
+    mine[row * L] = v;
+  };
   for (int r = 0; r < rounds; r += kAhead) {
 #pragma unroll
     for (int q = 0; q < kAhead; ++q) { e[q] = e_next[q]; g[q] = g_next[q]; d[q] = d_next[q]; }
@@ -173,11 +205,11 @@ __global__ void __launch_bounds__(kDuThreads) coef_d_u_kernel(const __grid_const
         twice |= other == e[q];
       }
       if (!__any_sync(0xffffffffu, have && twice)) {
-        if (have) mine[e[q] * L] = fmaf(g[q], d[q], mine[e[q] * L]);
+        if (have) add(e[q], g[q], d[q]);
       } else {
         const int turn = __popc(__match_any_sync(0xffffffffu, have ? e[q] : -1 - lane) & before);
         for (int w = 0; w < S; ++w) {
-          if (have && turn == w) mine[e[q] * L] = fmaf(g[q], d[q], mine[e[q] * L]);
+          if (have && turn == w) add(e[q], g[q], d[q]);
           __syncwarp();
         }
       }
@@ -185,32 +217,24 @@ __global__ void __launch_bounds__(kDuThreads) coef_d_u_kernel(const __grid_const
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < width; i += blockDim.x) {
+  // the kernel before this one in the stream (d_gates, whose output nothing here reads) may still run until here
+  ptx::griddep_wait();
+  const float *flat = reinterpret_cast<const float *>(tab);
+  for (int i = threadIdx.x; i < width * 4; i += blockDim.x) {
     float v = 0.f;
-    for (int q = 0; q < groups; ++q) v += tab[q * width + i];
-    const int x = i / L, q = i - x * L;
-    if (blockIdx.y * L + q < a.r1) a.partial[((int64_t)blockIdx.x * a.E + x) * a.r1 + blockIdx.y * L + q] = v;
+    for (int q = 0; q < groups; ++q) v += flat[q * width * 4 + i];
+    const int x = i / (L * 4), q = blockIdx.y * L * 4 + i - x * L * 4;
+    if (q < a.r1) a.partial[((int64_t)blockIdx.x * a.E + x) * a.r1 + q] = v;
   }
 }
 
 template <typename TU>
-__global__ void __launch_bounds__(256) coef_reduce_kernel(const float *__restrict__ partial, int blocks, int n, TU *__restrict__ d_u) {
-  __shared__ float part[8][33];
-  const int col = blockIdx.x * 32 + (threadIdx.x & 31), lane = threadIdx.x & 31, row = threadIdx.x >> 5;
+__global__ void __launch_bounds__(kColumnSumThreads) coef_reduce_kernel(const float *__restrict__ partial, int blocks, int n, TU *__restrict__ d_u) {
+  __shared__ float part[32][33];
+  const int col = blockIdx.x * 32 + (threadIdx.x & 31);
   ptx::griddep_wait();
-  float s = 0.f;
-  if (col < n) {
-#pragma unroll 4
-    for (int b = row; b < blocks; b += 8) s += partial[(int64_t)b * n + col];
-  }
-  part[row][lane] = s;
-  __syncthreads();
-  if (row == 0 && col < n) {
-    float t = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) t += part[i][lane];
-    d_u[col] = from_f32<TU>(t);
-  }
+  const float t = column_sum(partial, blocks, n, col, part);
+  if (threadIdx.x < 32 && col < n) d_u[col] = from_f32<TU>(t);
 }
 
 int check_coef(const tmoe_expert_coef_t *p) {
@@ -233,28 +257,27 @@ CoefArgs coef_args(const tmoe_expert_coef_t &p) {
   return a;
 }
 
-// Columns of a block (L), slots taken at once (S), groups with a table each, blocks over the tokens.  Tables of at most 32 KB leave room for
-// several groups; a group wants some rounds of work for the table it clears and folds.
+// Lanes over the columns of a block (4 columns each), slots taken at once, groups with a table each, blocks over the tokens.  Tables of at
+// most 32 KB leave room for several groups; a group wants some rounds of work for the table it clears and folds.
 struct DuShape { int L, S, parts, groups, blocks; };
 DuShape du_shape(int64_t T, int E, int k, int r1, int sms) {
   DuShape s;
   s.L = 1;
-  while (s.L < 32 && s.L < r1 && (int64_t)E * s.L * 2 * 4 <= 32 * 1024) s.L *= 2;
-  s.parts = (r1 + s.L - 1) / s.L;
+  while (s.L < 16 && s.L * 4 < r1 && (int64_t)E * s.L * 2 * 16 <= 32 * 1024) s.L *= 2;
+  s.parts = (r1 + s.L * 4 - 1) / (s.L * 4);
   s.S = 1;
   while (s.S < k && s.S * 2 * s.L <= 32) s.S *= 2;
-  const int most = (int)(kCoefSmem / ((int64_t)E * s.L * 4)), lanes = s.S * s.L;
+  const int most = (int)(kCoefSmem / ((int64_t)E * s.L * 16)), lanes = s.S * s.L, per_token = (k + s.S - 1) / s.S;
   const int64_t cap = (sms + s.parts - 1) / s.parts, want = (T + 31) / 32;
   s.blocks = (int)(want < cap ? want : cap);
-  const int64_t each = (T + s.blocks - 1) / s.blocks, rounds = 8 / ((k + s.S - 1) / s.S) > 0 ? 8 / ((k + s.S - 1) / s.S) : 1;
-  s.groups = (int)((each + rounds - 1) / rounds);
-  if (s.groups > most) s.groups = most;
+  const int64_t each = (T + s.blocks - 1) / s.blocks, tokens = per_token < 8 ? 8 / per_token : 1;
+  s.groups = (int)((each + tokens - 1) / tokens < most ? (each + tokens - 1) / tokens : most);
   if (s.groups > kDuThreads / lanes) s.groups = kDuThreads / lanes;
   return s;
 }
 
 template <int L>
-int launch_d_u(const CoefArgs &a, const DuShape &s, cudaStream_t st) {
+int launch_d_u(const CoefArgs &a, const DuShape &s, bool overlap, cudaStream_t st) {
   static std::atomic<uint64_t> opted{0};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return TMOE_ERR_CUDA;
@@ -263,9 +286,13 @@ int launch_d_u(const CoefArgs &a, const DuShape &s, cudaStream_t st) {
     if (cudaFuncSetAttribute(coef_d_u_kernel<L>, cudaFuncAttributeMaxDynamicSharedMemorySize, kCoefSmem) != cudaSuccess) return TMOE_ERR_CUDA;
     opted.fetch_or(bit, std::memory_order_relaxed);
   }
-  const int threads = (s.groups * s.S * s.L + 31) / 32 * 32;
-  coef_d_u_kernel<L><<<dim3(s.blocks, s.parts), threads, (size_t)s.groups * a.E * s.L * 4, st>>>(a, s.S, s.groups);
+  const int threads = (s.groups * s.S * s.L + 31) / 32 * 32, wide = a.r1 % 4 == 0 && !(reinterpret_cast<uintptr_t>(a.d_c) & 15);
+  const size_t smem = (size_t)s.groups * a.E * s.L * 16;
+  const dim3 grid((unsigned)s.blocks, (unsigned)s.parts), block((unsigned)threads);
   count_launch();
+  // after d_gates of the same call it may begin while that runs: both only read what was there before
+  if (overlap) return cuda_ok(launch_pdl(coef_d_u_kernel<L>, grid, block, smem, st, a, s.S, s.groups, wide));
+  coef_d_u_kernel<L><<<grid, block, smem, st>>>(a, s.S, s.groups, wide);
   return launch_status();
 }
 
@@ -273,12 +300,28 @@ int launch_d_u(const CoefArgs &a, const DuShape &s, cudaStream_t st) {
 bool cols_by_4(const CoefArgs &a, int size, const void *rows) {
   return a.r1 % 4 == 0 && !(reinterpret_cast<uintptr_t>(a.u) & (4 * size - 1)) && !(reinterpret_cast<uintptr_t>(rows) & 15);
 }
+// slots per 16- or 8-byte load of idx, gates and (backward) d_gates
+int slots_wide(const CoefArgs &a) {
+  const uintptr_t all = reinterpret_cast<uintptr_t>(a.idx) | reinterpret_cast<uintptr_t>(a.gates) | reinterpret_cast<uintptr_t>(a.d_gates);
+  return a.k % 4 == 0 && !(all & 15) ? 4 : a.k % 2 == 0 && !(all & 7) ? 2 : 1;
+}
+int spread(int64_t threads, int sms) {
+  const int64_t want = (threads + 255) / 256, cap = (int64_t)sms * 16;
+  return (int)(want < cap ? want : cap);
+}
 template <typename TU, int C>
-void launch_coef(const CoefArgs &a, int blocks, cudaStream_t st) {
-  const uintptr_t both = reinterpret_cast<uintptr_t>(a.idx) | reinterpret_cast<uintptr_t>(a.gates);
-  if (a.k % 4 == 0 && !(both & 15)) coef_kernel<TU, C, 4><<<blocks, 256, 0, st>>>(a);
-  else if (a.k % 2 == 0 && !(both & 7)) coef_kernel<TU, C, 2><<<blocks, 256, 0, st>>>(a);
+void launch_coef(const CoefArgs &a, int sms, cudaStream_t st) {
+  const int blocks = spread(a.T * (a.r1 / C), sms), kv = slots_wide(a);
+  if (kv == 4) coef_kernel<TU, C, 4><<<blocks, 256, 0, st>>>(a);
+  else if (kv == 2) coef_kernel<TU, C, 2><<<blocks, 256, 0, st>>>(a);
   else coef_kernel<TU, C, 1><<<blocks, 256, 0, st>>>(a);
+}
+template <typename TU, int C>
+void launch_d_gates(const CoefArgs &a, int sms, cudaStream_t st) {
+  const int kv = slots_wide(a), blocks = spread(a.T * (a.k / kv), sms);
+  if (kv == 4) coef_d_gates_kernel<TU, C, 4><<<blocks, 256, 0, st>>>(a);
+  else if (kv == 2) coef_d_gates_kernel<TU, C, 2><<<blocks, 256, 0, st>>>(a);
+  else coef_d_gates_kernel<TU, C, 1><<<blocks, 256, 0, st>>>(a);
 }
 
 }  // namespace
@@ -299,11 +342,9 @@ int tmoe_expert_coef(const tmoe_expert_coef_t *p, float *c, void *stream) {
   CoefArgs a = coef_args(*p);
   a.c = c;
   const bool four = cols_by_4(a, p->dtype == TMOE_F32 ? 4 : 2, c);
-  const int64_t want = (a.T * (a.r1 / (four ? 4 : 1)) + 255) / 256, cap = (int64_t)sms * 16;
-  const int blocks = (int)(want < cap ? want : cap);
   cudaStream_t st = (cudaStream_t)stream;
-  if (p->dtype == TMOE_F32) four ? launch_coef<float, 4>(a, blocks, st) : launch_coef<float, 1>(a, blocks, st);
-  else four ? launch_coef<bf16, 4>(a, blocks, st) : launch_coef<bf16, 1>(a, blocks, st);
+  if (p->dtype == TMOE_F32) four ? launch_coef<float, 4>(a, sms, st) : launch_coef<float, 1>(a, sms, st);
+  else four ? launch_coef<bf16, 4>(a, sms, st) : launch_coef<bf16, 1>(a, sms, st);
   count_launch();
   return launch_status();
 }
@@ -332,11 +373,9 @@ int tmoe_expert_coef_backward(const tmoe_expert_coef_t *p, const float *d_c, flo
   CoefArgs a = coef_args(*p);
   a.d_c = d_c; a.d_gates = d_gates;
   if (d_gates) {
-    const int64_t want = (a.T * a.k + 255) / 256, cap = (int64_t)sms * 16;
-    const int blocks = (int)(want < cap ? want : cap);
     const bool four = cols_by_4(a, size, d_c);
-    if (p->dtype == TMOE_F32) four ? coef_d_gates_kernel<float, 4><<<blocks, 256, 0, st>>>(a) : coef_d_gates_kernel<float, 1><<<blocks, 256, 0, st>>>(a);
-    else four ? coef_d_gates_kernel<bf16, 4><<<blocks, 256, 0, st>>>(a) : coef_d_gates_kernel<bf16, 1><<<blocks, 256, 0, st>>>(a);
+    if (p->dtype == TMOE_F32) four ? launch_d_gates<float, 4>(a, sms, st) : launch_d_gates<float, 1>(a, sms, st);
+    else four ? launch_d_gates<bf16, 4>(a, sms, st) : launch_d_gates<bf16, 1>(a, sms, st);
     count_launch();
     if ((rc = launch_status())) return rc;
   }
@@ -348,15 +387,14 @@ int tmoe_expert_coef_backward(const tmoe_expert_coef_t *p, const float *d_c, flo
     if (workspace_bytes < (int64_t)s.blocks * n * 4) return TMOE_ERR_WORKSPACE;
     a.partial = reinterpret_cast<float *>(workspace);
     switch (s.L) {
-      case 1: rc = launch_d_u<1>(a, s, st); break;
-      case 2: rc = launch_d_u<2>(a, s, st); break;
-      case 4: rc = launch_d_u<4>(a, s, st); break;
-      case 8: rc = launch_d_u<8>(a, s, st); break;
-      case 16: rc = launch_d_u<16>(a, s, st); break;
-      default: rc = launch_d_u<32>(a, s, st); break;
+      case 1: rc = launch_d_u<1>(a, s, d_gates != nullptr, st); break;
+      case 2: rc = launch_d_u<2>(a, s, d_gates != nullptr, st); break;
+      case 4: rc = launch_d_u<4>(a, s, d_gates != nullptr, st); break;
+      case 8: rc = launch_d_u<8>(a, s, d_gates != nullptr, st); break;
+      default: rc = launch_d_u<16>(a, s, d_gates != nullptr, st); break;
     }
     if (rc) return rc;
-    const dim3 grid((unsigned)((n + 31) / 32)), block(256);
+    const dim3 grid((unsigned)((n + 31) / 32)), block(kColumnSumThreads);
     rc = p->dtype == TMOE_F32 ? cuda_ok(launch_pdl(coef_reduce_kernel<float>, grid, block, 0, st, a.partial, s.blocks, n, (float *)d_U_expert))
                               : cuda_ok(launch_pdl(coef_reduce_kernel<bf16>, grid, block, 0, st, a.partial, s.blocks, n, (bf16 *)d_U_expert));
     count_launch();

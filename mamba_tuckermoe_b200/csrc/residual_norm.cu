@@ -22,6 +22,7 @@
 // layer_scale * S.
 // `out` is recomputed in fp32 from y, gate and residual (the same bytes as reading it back, and no rounding in between); only
 // the two rstd of a row are kept from the forward pass.
+#include "column_sum.cuh"
 #include "common.cuh"
 #include "kernels.h"
 #include "pair.cuh"
@@ -405,6 +406,7 @@ template <typename TY, typename TR, int VEC, int NV, bool GATE>
 __global__ void __launch_bounds__(32 * block_warps(VEC == 8 ? NV : NV / 8, true, sizeof(TY) == 4)) residual_norm_backward_kernel(const __grid_constant__ NormArgs a) {
   using In = RowIn<TY, TR, VEC, NV, GATE, true>;
   __shared__ __align__(16) TeamRed<3> red;
+  ptx::griddep_launch_dependents();
   red.init();
   const int tpr = a.tw * 32, team = threadIdx.x / tpr, lt = threadIdx.x - team * tpr, teams = blockDim.x / tpr;
   int row = blockIdx.x * teams + team;
@@ -519,22 +521,14 @@ __global__ void __launch_bounds__(32 * block_warps(VEC == 8 ? NV : NV / 8, true,
   }
 }
 
-// Sum of the blocks' partial rows, one column per thread column of a 32 x 8 block: each of the 8 rows of threads adds every
-// eighth block's value, then the eight are added in order and turned into the parameter gradients.
+// Adds the blocks' partial rows and turns the sums into the parameter gradients.
 template <typename TY>
-__global__ void __launch_bounds__(256) norm_params_kernel(const __grid_constant__ NormArgs a, int blocks, TY *d_ls, TY *d_w0, TY *d_w1) {
-  __shared__ float part[8][33];
-  const int lane = threadIdx.x & 31, col = blockIdx.x * 32 + lane, part_i = threadIdx.x >> 5;
-  const int n = a.n_sums * a.d;
-  float s = 0.f;
-  if (col < n)
-    for (int b = part_i; b < blocks; b += 8) s += a.partial[(int64_t)b * n + col];
-  part[part_i][lane] = s;
-  __syncthreads();
-  if (part_i == 0 && col < n) {
-    float t = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) t += part[i][lane];
+__global__ void __launch_bounds__(kColumnSumThreads) norm_params_kernel(const __grid_constant__ NormArgs a, int blocks, TY *d_ls, TY *d_w0, TY *d_w1) {
+  __shared__ float part[32][33];
+  const int col = blockIdx.x * 32 + (threadIdx.x & 31), n = a.n_sums * a.d;
+  ptx::griddep_wait();
+  const float t = column_sum(a.partial, blocks, n, col, part);
+  if (threadIdx.x < 32 && col < n) {
     const int which = col / a.d, e = col - which * a.d;
     if (which == a.sum_x) {
       d_w1[e] = from_f32<TY>(t);
@@ -749,13 +743,12 @@ int tmoe_residual_norm_backward(const tmoe_residual_norm_t *p, const float *rstd
   count_launch();
   if ((rc = launch_status())) return rc;
   if (params) {
-    const int grid = (a.n_sums * p->d + 31) / 32;
+    const dim3 grid((unsigned)((a.n_sums * p->d + 31) / 32)), block(kColumnSumThreads);
     if (p->dtype == TMOE_F32)
-      norm_params_kernel<float><<<grid, 256, 0, st>>>(a, s.blocks, (float *)d_layer_scale, (float *)d_post_w, (float *)d_next_w);
+      rc = cuda_ok(launch_pdl(norm_params_kernel<float>, grid, block, 0, st, a, s.blocks, (float *)d_layer_scale, (float *)d_post_w, (float *)d_next_w));
     else
-      norm_params_kernel<bf16><<<grid, 256, 0, st>>>(a, s.blocks, (bf16 *)d_layer_scale, (bf16 *)d_post_w, (bf16 *)d_next_w);
+      rc = cuda_ok(launch_pdl(norm_params_kernel<bf16>, grid, block, 0, st, a, s.blocks, (bf16 *)d_layer_scale, (bf16 *)d_post_w, (bf16 *)d_next_w));
     count_launch();
-    rc = launch_status();
   }
   return rc;
 }

@@ -412,7 +412,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_const
 // Sums the blocks' rows in a fixed order: counts, and the two losses.  One cluster of 8 blocks (one block alone took 45 us at 296 rows);
 // each takes an eighth of the columns, `width` threads side by side on them and the others on other rows, and block 0 puts the eight
 // parts of the balance loss together.
-constexpr int kLossBlocks = 8, kLossThreads = 512;
+constexpr int kLossBlocks = 8, kLossThreads = 1024;
 __global__ void __launch_bounds__(kLossThreads) route_losses_kernel(const __grid_constant__ RouteArgs a, int blocks, int width) {
   __shared__ float sp[kLossThreads];
   __shared__ int sc[kLossThreads];
@@ -430,7 +430,7 @@ __global__ void __launch_bounds__(kLossThreads) route_losses_kernel(const __grid
     float p = 0.f;
     int c = 0;
     if (in) {
-#pragma unroll 4
+#pragma unroll 8
       for (int b = slice; b < blocks; b += slices) {
         p += a.part_p[(int64_t)b * a.E + e];
         c += a.part_c[(int64_t)b * a.E + e];

@@ -105,7 +105,7 @@ def coef(**kw):
 
 @pytest.mark.parametrize("kw,code", [
     (dict(tokens=-1), SHAPE), (dict(n_experts=0), SHAPE), (dict(top_k=17), SHAPE), (dict(top_k=0), SHAPE), (dict(r1=0), SHAPE),
-    (dict(r1=65), SHAPE), (dict(n_experts=16385), UNSUPPORTED), (dict(dtype=9), DTYPE), (dict(idx=None), NULL), (dict(gates=None), NULL),
+    (dict(r1=65), SHAPE), (dict(n_experts=8193), UNSUPPORTED), (dict(dtype=9), DTYPE), (dict(idx=None), NULL), (dict(gates=None), NULL),
     (dict(U_expert=None), NULL), (dict(idx=P + 2), ALIGN), (dict(U_expert=P + 1), ALIGN),
 ])
 def test_coef_refusals(kw, code):

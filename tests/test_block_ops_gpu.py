@@ -485,7 +485,7 @@ def test_coef_sizes(T, E, k, r1):
 
 
 def test_coef_many_experts():
-    check_coef(*coef_inputs(50, 16384, 2, 4, F32))
+    check_coef(*coef_inputs(50, 8192, 2, 4, F32))
     check_coef(*coef_inputs(50, 1024, 2, 64, BF))
 
 
