@@ -23,37 +23,52 @@ __all__ = ["residual_norm", "route_tokens", "expert_coefficients", "Routing"]
 
 _DTYPES = {torch.float32: _lib.TMOE_F32, torch.bfloat16: _lib.TMOE_BF16}
 _is_compiling = torch.compiler.is_compiling
+_empty = torch.empty
+_F32, _I32, _U8 = torch.float32, torch.int32, torch.uint8
 
 
 def _fail(what: str):
     raise RuntimeError("tmoe_b200: " + what)
 
 
-class _on:
-    """Makes a tensor's device the current one (only when it is not) and gives its current stream's handle."""
-    __slots__ = ("index", "guard")
+def _call(device: torch.device, name: str, fn, *args):
+    """One C entry point on the device's current stream (its last argument).  The raw handle is read without building a Stream object:
+    a call at decode sizes costs more here than on the GPU."""
+    index = device.index
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc < 0:
+        _lib.check(rc, name)
 
-    def __init__(self, device: torch.device):
-        self.index, self.guard = device.index, None
 
-    def __enter__(self):
-        if torch.cuda.current_device() != self.index:
-            self.guard = torch.cuda.device(self.index)
-            self.guard.__enter__()
-        return torch.cuda.current_stream().cuda_stream
+def _first_order(backward):
+    """``once_differentiable`` where a graph of the gradients is being built, the plain function (several microseconds less) otherwise."""
+    guarded = once_differentiable(backward)
 
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+    def run(ctx, *grads):
+        return (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
+    return run
+
+
+def _size(name: str, fn, p) -> int:
+    n = fn(C.byref(p))
+    return n if n >= 0 else _lib.check(n, name)
 
 
 def _rows(t: torch.Tensor, width: int) -> torch.Tensor:
     """2-D view [rows, width] with contiguous rows (any row stride); copies only what cannot be viewed that way."""
     if t.dim() != 2:
         t = t.reshape(-1, width)
-    if t.stride(1) != 1 and width != 1 or t.stride(0) < 0:
+    if t.stride(1) != 1 and width != 1:
         t = t.contiguous()
     return t
+
+
+def _dense(t: torch.Tensor) -> torch.Tensor:
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _ptr(t: Optional[torch.Tensor]):
@@ -64,75 +79,86 @@ def _ptr(t: Optional[torch.Tensor]):
 def _check_norm(y, residual, gate, layer_scale, post_w, next_w):
     if not y.is_cuda:
         _fail("residual_norm runs on CUDA tensors only (no CPU fallback)")
-    if y.dtype not in _DTYPES:
-        _fail(f"unsupported dtype {y.dtype} (float32 and bfloat16 only)")
-    if y.dim() == 0:
+    dtype, shape, device = y.dtype, y.shape, y.device
+    if dtype not in _DTYPES:
+        _fail(f"unsupported dtype {dtype} (float32 and bfloat16 only)")
+    if not shape:
         _fail("y must be (..., d)")
-    d = y.shape[-1]
-    if residual is not None and (residual.shape != y.shape or residual.device != y.device or
-                                 (residual.dtype != y.dtype and residual.dtype != torch.float32)):
+    if residual is not None and (residual.shape != shape or residual.device != device or
+                                 (residual.dtype != dtype and residual.dtype != _F32)):
         _fail("residual must have y's shape and device and y's dtype or float32")
-    if gate is not None and (gate.shape != y.shape or gate.dtype != y.dtype or gate.device != y.device):
+    if gate is not None and (gate.shape != shape or gate.dtype != dtype or gate.device != device):
         _fail("gate must have y's shape, dtype and device")
-    for name, w in (("layer_scale", layer_scale), ("post_norm weight", post_w), ("next_norm weight", next_w)):
-        if w is not None and (w.shape != (d,) or w.dtype != y.dtype or w.device != y.device):
-            _fail(f"{name} must be (d,) in y's dtype on its device")
+    d = shape[-1]
+    for w in (layer_scale, post_w, next_w):
+        if w is not None and (w.dim() != 1 or w.shape[0] != d or w.dtype != dtype or w.device != device):
+            _fail("layer_scale and the norm weights must be (d,) in y's dtype on its device")
     return d
 
 
-def _norm_struct(y2, res2, gate2, layer_scale, post_w, next_w, post_eps, next_eps) -> ResidualNorm:
-    rows, d = y2.shape
-    dt = _DTYPES[y2.dtype]
-    return ResidualNorm(rows, d, dt, dt if res2 is None else _DTYPES[res2.dtype], post_eps, next_eps, 0, y2.stride(0),
-                        0 if res2 is None else res2.stride(0), 0 if gate2 is None else gate2.stride(0), y2.data_ptr(),
-                        _ptr(res2), _ptr(gate2), _ptr(layer_scale), _ptr(post_w), _ptr(next_w))
+def _norm_struct(y, residual, gate, layer_scale, post_w, next_w, post_eps, next_eps):
+    """(struct, tensors that must outlive the call)"""
+    d = y.shape[-1]
+    y2 = _rows(y, d)
+    dt = _DTYPES[y.dtype]
+    res_dt, res_stride, gate_stride, res2, gate2 = dt, 0, 0, None, None
+    if residual is not None:
+        res2 = _rows(residual, d)
+        res_dt, res_stride = _DTYPES[residual.dtype], res2.stride(0)
+    if gate is not None:
+        gate2 = _rows(gate, d)
+        gate_stride = gate2.stride(0)
+    keep = [y2, res2, gate2]
+    ptrs = []
+    for w in (layer_scale, post_w, next_w):
+        if w is not None:
+            w = _dense(w)
+            keep.append(w)
+            ptrs.append(w.data_ptr())
+        else:
+            ptrs.append(None)
+    return ResidualNorm(y2.shape[0], d, dt, res_dt, post_eps, next_eps, 0, y2.stride(0), res_stride, gate_stride, y2.data_ptr(),
+                        _ptr(res2), _ptr(gate2), *ptrs), keep
 
 
 def _norm_forward(y, residual, gate, layer_scale, post_w, next_w, post_eps, next_eps, keep):
     """(out or None, normed or None, rstd or None); out is None where it would be y."""
-    d = _check_norm(y, residual, gate, layer_scale, post_w, next_w)
-    shape = y.shape
-    y2 = _rows(y, d)
-    rows = y2.shape[0]
-    res2 = None if residual is None else _rows(residual, d)
-    gate2 = None if gate is None else _rows(gate, d)
-    layer_scale, post_w, next_w = (w if w is None or w.is_contiguous() else w.contiguous() for w in (layer_scale, post_w, next_w))
-    changed = residual is not None or gate is not None or layer_scale is not None or post_w is not None
-    out = torch.empty(shape, dtype=y.dtype if residual is None else residual.dtype, device=y.device) if changed else None
-    normed = torch.empty(shape, dtype=y.dtype, device=y.device) if next_w is not None else None
-    rstd = torch.empty((2, rows), dtype=torch.float32, device=y.device) if keep else None
-    p = _norm_struct(y2, res2, gate2, layer_scale, post_w, next_w, post_eps, next_eps)
-    lib = _lib.load()
-    with _on(y.device) as stream:
-        rc = lib.tmoe_residual_norm(C.byref(p), _ptr(out), _ptr(normed), _ptr(rstd), stream)
-    if rc < 0:
-        _lib.check(rc, "tmoe_residual_norm")
+    _check_norm(y, residual, gate, layer_scale, post_w, next_w)
+    p, held = _norm_struct(y, residual, gate, layer_scale, post_w, next_w, post_eps, next_eps)
+    shape, device = y.shape, y.device
+    out = normed = rstd = None
+    if residual is not None:
+        out = _empty(shape, dtype=residual.dtype, device=device)
+    elif gate is not None or layer_scale is not None or post_w is not None:
+        out = _empty(shape, dtype=y.dtype, device=device)
+    if next_w is not None:
+        normed = _empty(shape, dtype=y.dtype, device=device)
+    if keep:
+        rstd = _empty((2, p.rows), dtype=_F32, device=device)
+    _call(device, "tmoe_residual_norm", _lib.load().tmoe_residual_norm, C.byref(p), _ptr(out), _ptr(normed), _ptr(rstd))
     return out, normed, rstd
 
 
 def _norm_backward(y, residual, gate, layer_scale, post_w, next_w, post_eps, next_eps, rstd, d_out, d_normed, want):
     """Gradients of (y, residual, gate, layer_scale, post_w, next_w) where `want` says so, None elsewhere."""
-    d = y.shape[-1]
-    y2 = _rows(y, d)
-    rows = y2.shape[0]
-    res2 = None if residual is None else _rows(residual, d)
-    gate2 = None if gate is None else _rows(gate, d)
-    layer_scale, post_w, next_w = (w if w is None or w.is_contiguous() else w.contiguous() for w in (layer_scale, post_w, next_w))
-    do2 = None if d_out is None else _rows(d_out, d)
-    dn2 = None if d_normed is None else _rows(d_normed, d)
-    grads = [torch.empty(t.shape, dtype=t.dtype, device=y.device) if w else None
+    p, held = _norm_struct(y, residual, gate, layer_scale, post_w, next_w, post_eps, next_eps)
+    d, device = p.d, y.device
+    do2 = dn2 = None
+    do_stride = dn_stride = 0
+    if d_out is not None:
+        do2 = _rows(d_out, d)
+        do_stride = do2.stride(0)
+    if d_normed is not None:
+        dn2 = _rows(d_normed, d)
+        dn_stride = dn2.stride(0)
+    grads = [_empty(t.shape, dtype=t.dtype, device=device) if w else None
              for t, w in zip((y, residual, gate, layer_scale, post_w, next_w), want)]
-    p = _norm_struct(y2, res2, gate2, layer_scale, post_w, next_w, post_eps, next_eps)
-    lib = _lib.load()
-    with _on(y.device) as stream:
-        ws, n = None, 0
-        if want[3] or want[4] or want[5]:
-            n = _lib.check(lib.tmoe_residual_norm_workspace_bytes(C.byref(p)), "tmoe_residual_norm_workspace_bytes")
-            ws = torch.empty(n, dtype=torch.uint8, device=y.device)
-        rc = lib.tmoe_residual_norm_backward(C.byref(p), _ptr(rstd), _ptr(do2), 0 if do2 is None else do2.stride(0), _ptr(dn2),
-                                             0 if dn2 is None else dn2.stride(0), *map(_ptr, grads), _ptr(ws), n, stream)
-    if rc < 0:
-        _lib.check(rc, "tmoe_residual_norm_backward")
+    lib, ws, n = _lib.load(), None, 0
+    if want[3] or want[4] or want[5]:
+        n = _size("tmoe_residual_norm_workspace_bytes", lib.tmoe_residual_norm_workspace_bytes, p)
+        ws = _empty(n, dtype=_U8, device=device)
+    _call(device, "tmoe_residual_norm_backward", lib.tmoe_residual_norm_backward, C.byref(p), _ptr(rstd), _ptr(do2), do_stride,
+          _ptr(dn2), dn_stride, *[None if g is None else g.data_ptr() for g in grads], _ptr(ws), n)
     return grads
 
 
@@ -146,7 +172,7 @@ class _ResidualNorm(torch.autograd.Function):
         return out, normed
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, d_out, d_normed):
         if d_out is None and d_normed is None:
             return (None,) * 8
@@ -209,7 +235,16 @@ torch.library.register_autograd("tmoe_b200::residual_norm", _norm_op_backward, s
 def _weight_eps(norm):
     if norm is None:
         return None, 0.0
-    return (norm.weight, float(norm.eps)) if hasattr(norm, "weight") else (norm[0], float(norm[1]))
+    if type(norm) is not tuple and hasattr(norm, "weight"):
+        return norm.weight, float(norm.eps)
+    return norm[0], float(norm[1])
+
+
+def _wants_grad(*tensors) -> bool:
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            return True
+    return False
 
 
 def residual_norm(y: torch.Tensor, *, residual: Optional[torch.Tensor] = None, layer_scale: Optional[torch.Tensor] = None,
@@ -232,14 +267,13 @@ def residual_norm(y: torch.Tensor, *, residual: Optional[torch.Tensor] = None, l
     changed = residual is not None or gate is not None or layer_scale is not None or post_w is not None
     if not changed and next_w is None:
         _fail("residual_norm has nothing to do: give it a residual, layer_scale, gate, post_norm or next_norm")
-    ins = (y, residual, gate, layer_scale, post_w, next_w)
     if _is_compiling():
-        out, normed, _ = torch.ops.tmoe_b200.residual_norm(*ins, post_eps, next_eps)
+        out, normed, _ = torch.ops.tmoe_b200.residual_norm(y, residual, gate, layer_scale, post_w, next_w, post_eps, next_eps)
         return out if changed else y, normed if next_w is not None else None
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ins):
-        out, normed = _ResidualNorm.apply(*ins, post_eps, next_eps)
+    if torch.is_grad_enabled() and (y.requires_grad or _wants_grad(residual, gate, layer_scale, post_w, next_w)):
+        out, normed = _ResidualNorm.apply(y, residual, gate, layer_scale, post_w, next_w, post_eps, next_eps)
     else:
-        out, normed, _ = _norm_forward(*ins, post_eps, next_eps, False)
+        out, normed, _ = _norm_forward(y, residual, gate, layer_scale, post_w, next_w, post_eps, next_eps, False)
     return out if changed else y, normed
 
 
@@ -264,48 +298,42 @@ def _check_route(scores, top_k, mask):
         _fail("token_mask must be a bool tensor of scores.shape[:-1] on its device")
 
 
-def _route_struct(s2, mask, top_k, router) -> Route:
-    return Route(s2.shape[0], s2.shape[1], top_k, _DTYPES[s2.dtype], router[0], router[1], router[2], s2.stride(0), s2.data_ptr(),
-                 _ptr(mask))
+def _route_struct(scores, mask, top_k, router):
+    """(struct, tensors that must outlive the call)"""
+    E = scores.shape[-1]
+    s2 = _rows(scores, E)
+    if mask is not None:
+        mask = _dense(mask)
+    return Route(s2.shape[0], E, top_k, _DTYPES[s2.dtype], router[0], router[1], router[2], s2.stride(0), s2.data_ptr(),
+                 _ptr(mask)), (s2, mask)
 
 
 def _route_forward(scores, mask, top_k, router, keep=False):
     """(idx, gates, counts, losses, stats or None)"""
     _check_route(scores, top_k, mask)
-    E, lead, dev = scores.shape[-1], scores.shape[:-1], scores.device
-    s2 = _rows(scores, E)
-    if mask is not None and not mask.is_contiguous():
-        mask = mask.contiguous()
-    idx = torch.empty((*lead, top_k), dtype=torch.int32, device=dev)
-    gates = torch.empty((*lead, top_k), dtype=torch.float32, device=dev)
-    counts = torch.empty(E, dtype=torch.int32, device=dev)
-    losses = torch.empty(3, dtype=torch.float32, device=dev)
-    stats = torch.empty((*lead, 2), dtype=torch.float32, device=dev) if keep else None
-    p = _route_struct(s2, mask, top_k, router)
+    p, held = _route_struct(scores, mask, top_k, router)
+    slots, dev = (*scores.shape[:-1], top_k), scores.device
+    idx = _empty(slots, dtype=_I32, device=dev)
+    gates = _empty(slots, dtype=_F32, device=dev)
+    counts = _empty(scores.shape[-1], dtype=_I32, device=dev)
+    losses = _empty(3, dtype=_F32, device=dev)
+    stats = _empty((p.tokens, 2), dtype=_F32, device=dev) if keep else None
     lib = _lib.load()
-    with _on(dev) as stream:
-        n = _lib.check(lib.tmoe_route_workspace_bytes(C.byref(p)), "tmoe_route_workspace_bytes")
-        ws = torch.empty(n, dtype=torch.uint8, device=dev)
-        rc = lib.tmoe_route_tokens(C.byref(p), idx.data_ptr(), gates.data_ptr(), counts.data_ptr(), losses.data_ptr(), _ptr(stats),
-                                   ws.data_ptr(), n, stream)
-    if rc < 0:
-        _lib.check(rc, "tmoe_route_tokens")
+    n = _size("tmoe_route_workspace_bytes", lib.tmoe_route_workspace_bytes, p)
+    ws = _empty(n, dtype=_U8, device=dev)
+    _call(dev, "tmoe_route_tokens", lib.tmoe_route_tokens, C.byref(p), idx.data_ptr(), gates.data_ptr(), counts.data_ptr(),
+          losses.data_ptr(), _ptr(stats), ws.data_ptr(), n)
     return idx, gates, counts, losses, stats
 
 
 def _route_backward(scores, mask, idx, gates, counts, losses, stats, top_k, router, d_gates, d_balance, d_z):
-    E = scores.shape[-1]
-    s2 = _rows(scores, E)
-    if mask is not None and not mask.is_contiguous():
-        mask = mask.contiguous()
-    d_gates, d_balance, d_z = (g if g is None else g.to(torch.float32).contiguous() for g in (d_gates, d_balance, d_z))
-    d_scores = torch.empty(scores.shape, dtype=scores.dtype, device=scores.device)
-    p = _route_struct(s2, mask, top_k, router)
-    with _on(scores.device) as stream:
-        rc = _lib.load().tmoe_route_tokens_backward(C.byref(p), idx.data_ptr(), gates.data_ptr(), counts.data_ptr(), losses.data_ptr(),
-                                                    stats.data_ptr(), _ptr(d_gates), _ptr(d_balance), _ptr(d_z), d_scores.data_ptr(), stream)
-    if rc < 0:
-        _lib.check(rc, "tmoe_route_tokens_backward")
+    p, held = _route_struct(scores, mask, top_k, router)
+    if d_gates is not None:
+        d_gates = _dense(d_gates)
+    d_scores = _empty(scores.shape, dtype=scores.dtype, device=scores.device)
+    _call(scores.device, "tmoe_route_tokens_backward", _lib.load().tmoe_route_tokens_backward, C.byref(p), idx.data_ptr(),
+          gates.data_ptr(), counts.data_ptr(), losses.data_ptr(), stats.data_ptr(), _ptr(d_gates), _ptr(d_balance), _ptr(d_z),
+          d_scores.data_ptr())
     return d_scores
 
 
@@ -317,10 +345,10 @@ class _RouteTokens(torch.autograd.Function):
         ctx.mark_non_differentiable(idx, counts)
         ctx.save_for_backward(scores, mask, idx, gates, counts, losses, stats)
         ctx.top_k, ctx.router = top_k, router
-        return idx, gates, counts, losses[0].clone(), losses[1].clone()
+        return idx, gates, counts, losses[0], losses[1]
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, d_idx, d_gates, d_counts, d_balance, d_z):
         if d_gates is None and d_balance is None and d_z is None:
             return None, None, None, None
@@ -339,7 +367,7 @@ def _(scores, mask, top_k, router_mode, router_cap, router_temperature):
     return (scores.new_empty((*scores.shape[:-1], top_k), dtype=torch.int32),
             scores.new_empty((*scores.shape[:-1], top_k), dtype=torch.float32),
             scores.new_empty((scores.shape[-1],), dtype=torch.int32), scores.new_empty((3,), dtype=torch.float32),
-            scores.new_empty((*scores.shape[:-1], 2), dtype=torch.float32))
+            scores.new_empty((scores.numel() // max(scores.shape[-1], 1), 2), dtype=torch.float32))
 
 
 @torch.library.custom_op("tmoe_b200::route_tokens_backward", mutates_args=())
@@ -407,37 +435,33 @@ def _check_coef(idx, gates, U_expert):
         _fail("idx, gates and U_expert must be on one device")
 
 
-def _coef_struct(idx, gates, u) -> ExpertCoef:
+def _coef_struct(idx, gates, u):
+    """(struct, tensors that must outlive the call)"""
+    idx, gates, u = _dense(idx), _dense(gates), _dense(u)
     k = idx.shape[-1]
-    return ExpertCoef(idx.numel() // k if k else 0, u.shape[0], k, u.shape[1], _DTYPES[u.dtype], idx.data_ptr(), gates.data_ptr(), u.data_ptr())
+    return ExpertCoef(idx.numel() // k if k else 0, u.shape[0], k, u.shape[1], _DTYPES[u.dtype], idx.data_ptr(), gates.data_ptr(),
+                      u.data_ptr()), (idx, gates, u)
 
 
 def _coef_forward(idx, gates, u):
     _check_coef(idx, gates, u)
-    idx, gates, u = (t if t.is_contiguous() else t.contiguous() for t in (idx, gates, u))
-    c = torch.empty((*idx.shape[:-1], u.shape[1]), dtype=torch.float32, device=u.device)
-    p = _coef_struct(idx, gates, u)
-    with _on(u.device) as stream:
-        rc = _lib.load().tmoe_expert_coef(C.byref(p), c.data_ptr(), stream)
-    if rc < 0:
-        _lib.check(rc, "tmoe_expert_coef")
+    p, held = _coef_struct(idx, gates, u)
+    c = _empty((*idx.shape[:-1], u.shape[1]), dtype=_F32, device=u.device)
+    _call(u.device, "tmoe_expert_coef", _lib.load().tmoe_expert_coef, C.byref(p), c.data_ptr())
     return c
 
 
 def _coef_backward(idx, gates, u, d_c, want_gates, want_u):
-    idx, gates, u, d_c = (t if t.is_contiguous() else t.contiguous() for t in (idx, gates, u, d_c))
-    d_gates = torch.empty(gates.shape, dtype=torch.float32, device=u.device) if want_gates else None
-    d_u = torch.empty(u.shape, dtype=u.dtype, device=u.device) if want_u else None
-    p = _coef_struct(idx, gates, u)
-    lib = _lib.load()
-    with _on(u.device) as stream:
-        ws, n = None, 0
-        if want_u:
-            n = _lib.check(lib.tmoe_expert_coef_workspace_bytes(C.byref(p)), "tmoe_expert_coef_workspace_bytes")
-            ws = torch.empty(n, dtype=torch.uint8, device=u.device)
-        rc = lib.tmoe_expert_coef_backward(C.byref(p), d_c.data_ptr(), _ptr(d_gates), _ptr(d_u), _ptr(ws), n, stream)
-    if rc < 0:
-        _lib.check(rc, "tmoe_expert_coef_backward")
+    p, held = _coef_struct(idx, gates, u)
+    d_c, dev = _dense(d_c), u.device
+    d_gates = _empty(gates.shape, dtype=_F32, device=dev) if want_gates else None
+    lib, d_u, ws, n = _lib.load(), None, None, 0
+    if want_u:
+        d_u = _empty(u.shape, dtype=u.dtype, device=dev)
+        n = _size("tmoe_expert_coef_workspace_bytes", lib.tmoe_expert_coef_workspace_bytes, p)
+        ws = _empty(n, dtype=_U8, device=dev)
+    _call(dev, "tmoe_expert_coef_backward", lib.tmoe_expert_coef_backward, C.byref(p), d_c.data_ptr(), _ptr(d_gates), _ptr(d_u),
+          _ptr(ws), n)
     return d_gates, d_u
 
 
@@ -448,7 +472,7 @@ class _ExpertCoefficients(torch.autograd.Function):
         return _coef_forward(idx, gates, u)
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, d_c):
         return (None, *_coef_backward(*ctx.saved_tensors, d_c, ctx.needs_input_grad[1], ctx.needs_input_grad[2]))
 
@@ -460,7 +484,7 @@ def _coef_op(idx: torch.Tensor, gates: torch.Tensor, U_expert: torch.Tensor) -> 
 
 @_coef_op.register_fake
 def _(idx, gates, U_expert):
-    return gates.new_empty((*idx.shape[:-1], U_expert.shape[1]))
+    return gates.new_empty((*idx.shape[:-1], U_expert.shape[1]), dtype=torch.float32)
 
 
 @torch.library.custom_op("tmoe_b200::expert_coefficients_backward", mutates_args=())

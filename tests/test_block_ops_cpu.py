@@ -149,7 +149,7 @@ def test_fake_operators_give_shapes_without_a_gpu():
         g = torch.ops.tmoe_b200.residual_norm_backward(y, res, None, w, None, w, 1e-5, 1e-5, rstd, out, normed)
         assert [t.shape for t in g] == [y.shape, res.shape, w.shape, w.shape]
         idx, gates, counts, losses, stats = torch.ops.tmoe_b200.route_tokens(torch.empty(3, 7, 40), None, 2, 0, 10.0, 0.5)
-        assert idx.shape == gates.shape == (3, 7, 2) and idx.dtype == counts.dtype == torch.int32 and counts.shape == (40,) and losses.shape == (3,) and stats.shape == (3, 7, 2)
+        assert idx.shape == gates.shape == (3, 7, 2) and idx.dtype == counts.dtype == torch.int32 and counts.shape == (40,) and losses.shape == (3,) and stats.shape == (21, 2)
         assert torch.ops.tmoe_b200.expert_coefficients(idx, gates, torch.empty(40, 6)).shape == (3, 7, 6)
 
 
