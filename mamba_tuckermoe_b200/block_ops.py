@@ -71,6 +71,11 @@ def _dense(t: torch.Tensor) -> torch.Tensor:
     return t if t.is_contiguous() else t.contiguous()
 
 
+def _like(t: torch.Tensor) -> torch.Tensor:
+    """A dense tensor of t's shape and dtype (``empty_like`` of a dense one costs half of ``empty`` with its arguments)."""
+    return torch.empty_like(t) if t.is_contiguous() else _empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
@@ -125,14 +130,13 @@ def _norm_forward(y, residual, gate, layer_scale, post_w, next_w, post_eps, next
     """(out or None, normed or None, rstd or None); out is None where it would be y."""
     _check_norm(y, residual, gate, layer_scale, post_w, next_w)
     p, held = _norm_struct(y, residual, gate, layer_scale, post_w, next_w, post_eps, next_eps)
-    shape, device = y.shape, y.device
-    out = normed = rstd = None
+    device, out, normed, rstd = y.device, None, None, None
     if residual is not None:
-        out = _empty(shape, dtype=residual.dtype, device=device)
+        out = _like(residual)
     elif gate is not None or layer_scale is not None or post_w is not None:
-        out = _empty(shape, dtype=y.dtype, device=device)
+        out = _like(y)
     if next_w is not None:
-        normed = _empty(shape, dtype=y.dtype, device=device)
+        normed = _like(y)
     if keep:
         rstd = _empty((2, p.rows), dtype=_F32, device=device)
     _call(device, "tmoe_residual_norm", _lib.load().tmoe_residual_norm, C.byref(p), _ptr(out), _ptr(normed), _ptr(rstd))
@@ -151,8 +155,7 @@ def _norm_backward(y, residual, gate, layer_scale, post_w, next_w, post_eps, nex
     if d_normed is not None:
         dn2 = _rows(d_normed, d)
         dn_stride = dn2.stride(0)
-    grads = [_empty(t.shape, dtype=t.dtype, device=device) if w else None
-             for t, w in zip((y, residual, gate, layer_scale, post_w, next_w), want)]
+    grads = [_like(t) if w else None for t, w in zip((y, residual, gate, layer_scale, post_w, next_w), want)]
     lib, ws, n = _lib.load(), None, 0
     if want[3] or want[4] or want[5]:
         n = _size("tmoe_residual_norm_workspace_bytes", lib.tmoe_residual_norm_workspace_bytes, p)
@@ -330,7 +333,7 @@ def _route_backward(scores, mask, idx, gates, counts, losses, stats, top_k, rout
     p, held = _route_struct(scores, mask, top_k, router)
     if d_gates is not None:
         d_gates = _dense(d_gates)
-    d_scores = _empty(scores.shape, dtype=scores.dtype, device=scores.device)
+    d_scores = _like(scores)
     _call(scores.device, "tmoe_route_tokens_backward", _lib.load().tmoe_route_tokens_backward, C.byref(p), idx.data_ptr(),
           gates.data_ptr(), counts.data_ptr(), losses.data_ptr(), stats.data_ptr(), _ptr(d_gates), _ptr(d_balance), _ptr(d_z),
           d_scores.data_ptr())
@@ -454,10 +457,10 @@ def _coef_forward(idx, gates, u):
 def _coef_backward(idx, gates, u, d_c, want_gates, want_u):
     p, held = _coef_struct(idx, gates, u)
     d_c, dev = _dense(d_c), u.device
-    d_gates = _empty(gates.shape, dtype=_F32, device=dev) if want_gates else None
+    d_gates = _like(gates) if want_gates else None
     lib, d_u, ws, n = _lib.load(), None, None, 0
     if want_u:
-        d_u = _empty(u.shape, dtype=u.dtype, device=dev)
+        d_u = _like(u)
         n = _size("tmoe_expert_coef_workspace_bytes", lib.tmoe_expert_coef_workspace_bytes, p)
         ws = _empty(n, dtype=_U8, device=dev)
     _call(dev, "tmoe_expert_coef_backward", lib.tmoe_expert_coef_backward, C.byref(p), d_c.data_ptr(), _ptr(d_gates), _ptr(d_u),
