@@ -14,7 +14,6 @@ import ctypes as C
 from typing import NamedTuple, Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import ExpertCoef, ResidualNorm, Route
@@ -44,12 +43,27 @@ def _call(device: torch.device, name: str, fn, *args):
         _lib.check(rc, name)
 
 
-def _first_order(backward):
-    """``once_differentiable`` where a graph of the gradients is being built, the plain function (several microseconds less) otherwise."""
-    guarded = once_differentiable(backward)
+class _FirstOrderOnly(torch.autograd.Function):
+    """A gradient that depends on ``anchors`` in a way that has no formula here: differentiating it is an error, not a zero."""
 
+    @staticmethod
+    def forward(ctx, grad, *anchors):
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, *_):
+        _fail("gradients of gradients are not implemented")
+
+
+def _first_order(backward):
+    """A custom function's backward, whose results refuse to be differentiated where a graph of the gradients is being built."""
     def run(ctx, *grads):
-        return (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
+        if not torch.is_grad_enabled():
+            return backward(ctx, *grads)
+        with torch.no_grad():
+            got = backward(ctx, *grads)
+        anchors = [t for t in (*ctx.saved_tensors, *grads) if t is not None and t.requires_grad]
+        return tuple(g if g is None else _FirstOrderOnly.apply(g, *anchors) for g in got)
     return run
 
 

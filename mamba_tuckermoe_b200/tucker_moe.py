@@ -19,6 +19,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib
+from .block_ops import residual_norm
 from ._lib import PATH_AUTO, PATH_DECODE, PATH_SIMT, PATH_TENSOR, Extras, Factors, Layer
 
 __all__ = ["TuckerMoE", "TuckerMoEConfig", "RMSNorm", "tucker_moe_forward", "tucker_moe_forward_taps", "prepare_factors",
@@ -534,15 +535,33 @@ class TuckerMoE(nn.Module):
 
     def forward_fused(self, x: torch.Tensor, *, pre_norm=None, residual: Optional[torch.Tensor] = None,
                       layer_scale: Optional[torch.Tensor] = None, silu_gate: Optional[torch.Tensor] = None,
-                      return_routing: bool = False):
+                      return_routing: bool = False, post_norm=None, next_norm=None):
         """The layer with the callers' element-wise work attached:
 
         ``pre_norm``  an RMSNorm module (anything with ``.weight`` and ``.eps``) or a ``(weight, eps)`` pair
                       applied to ``x`` first (``norm_out_proj`` / ``norm_ffn``, ``model.py:258, 337``);
+        ``post_norm`` the same, applied to the layer's output before the gate and the residual;
         ``silu_gate`` ``silu(silu_gate) * layer(...)`` in the out-projection's epilogue (``model.py:340``);
-        ``residual``, ``layer_scale``  ``residual + layer_scale * (...)`` in the same epilogue (``model.py:260, 341``).
+        ``residual``, ``layer_scale``  ``residual + layer_scale * (...)`` in the same epilogue (``model.py:260, 341``);
+        ``next_norm`` the norm in front of the next block: the result becomes ``(out, next_norm(out))``.
         ``return_routing``  also return ``(idx, gates, c)`` of the call (same kernels, same output).
+
+        A norm behind the layer needs whole rows, so with ``post_norm`` the tail is one pass of ``residual_norm`` over the
+        layer's output (there ``residual`` may come without ``layer_scale``, and in float32); without it the tail stays in
+        the GEMM's epilogue and ``next_norm`` is one pass over the result, which moves less.
         """
+        if post_norm is not None or next_norm is not None:
+            tail = {} if post_norm is not None else dict(residual=residual, layer_scale=layer_scale, silu_gate=silu_gate)
+            y = self.forward_fused(x, pre_norm=pre_norm, return_routing=return_routing, **tail)
+            y, routing = y if return_routing else (y, None)
+            if post_norm is not None:
+                y = residual_norm(y, residual=residual, layer_scale=layer_scale, gate=silu_gate, post_norm=post_norm,
+                                  next_norm=next_norm)
+                y = y if next_norm is not None else y[0]
+            else:
+                w, e = (next_norm.weight, next_norm.eps) if hasattr(next_norm, "weight") else next_norm
+                y = (y, rms_norm(y, w, e))
+            return (y, routing) if return_routing else y
         if pre_norm is not None and hasattr(pre_norm, "weight"):
             pre_norm = (pre_norm.weight, pre_norm.eps)
         if (residual is None) != (layer_scale is None):
@@ -586,6 +605,37 @@ class TuckerMoE(nn.Module):
         return tucker_moe_forward(x, rw, ui, nw, self.inner_norm.eps, ue, co, uo, b, self.top_k, path=self.path,
                                   residual=residual, layer_scale=layer_scale, prepared=self._prepared_for(x),
                                   router=self._router())
+
+    @torch.no_grad()
+    def forward_routed(self, x: torch.Tensor, c: torch.Tensor) -> torch.Tensor:
+        """The layer on routing made outside: ``c`` (..., r1) float32 are the coefficients that mix the core slices
+        (``expert_coefficients`` of ``route_tokens``' choice, say with some experts switched off or tokens masked).  Everything
+        but the router is the layer's own: the in-projection / core and out-projection stages on the tensor cores where they
+        cover it, else on the CUDA cores.  Like ``forward`` the result carries no autograd graph, so neither ``x`` nor ``c``
+        gets a gradient through it."""
+        ps = self._params()
+        _validate(x, ps, self.top_k)
+        d_in, d_out, (r1, _, r2) = self.U_in.shape[0], self.U_out.shape[1], self.core.shape
+        if c.shape != (*x.shape[:-1], r1) or c.dtype != torch.float32 or c.device != x.device:
+            raise RuntimeError("tmoe_b200: c must be float32 (..., r1) with x's leading shape on x's device")
+        x2, c2 = x.reshape(-1, d_in), c.reshape(-1, r1)
+        x2, c2 = (t if t.is_contiguous() and not t.data_ptr() & 15 else t.contiguous().clone() for t in (x2, c2))
+        T, dev = x2.shape[0], x.device
+        y = torch.empty((T, d_out), dtype=x.dtype, device=dev)
+        if T:
+            plan = self._plan_for(x)
+            lib = plan.lib
+            with torch.cuda.device(dev):
+                stream = torch.cuda.current_stream(dev).cuda_stream
+                # the decode kernels have no stages of their own
+                path = PATH_SIMT if self.path == PATH_SIMT or lib.tmoe_resolve_path(plan.layer_ref, T, PATH_TENSOR) < 0 else PATH_TENSOR
+                ws = _workspace(dev, _lib.check(lib.tmoe_workspace_bytes(plan.layer_ref, T, path), "tmoe_workspace_bytes"), stream)
+                z = torch.empty((T, r2), dtype=torch.float32 if path == PATH_SIMT else x.dtype, device=dev)
+                _lib.check(lib.tmoe_in_core(plan.layer_ref, plan.factors_ref, plan.prepared_ptr, x2.data_ptr(), T, c2.data_ptr(),
+                                            z.data_ptr(), ws.data_ptr(), ws.numel(), path, stream), "tmoe_in_core")
+                _lib.check(lib.tmoe_out(plan.layer_ref, plan.factors_ref, plan.prepared_ptr, z.data_ptr(), T, y.data_ptr(), None,
+                                        ws.data_ptr(), ws.numel(), path, stream), "tmoe_out")
+        return y.reshape(*x.shape[:-1], d_out)
 
     def forward_with_routing(self, x: torch.Tensor):
         rw, ui, nw, ue, co, uo, b = self._params()
@@ -686,10 +736,11 @@ class TuckerMoE(nn.Module):
         return state
 
 
-def fused_out_proj(out_proj: TuckerMoE, mid: torch.Tensor, norm, layer_scale: torch.Tensor) -> torch.Tensor:
+def fused_out_proj(out_proj: TuckerMoE, mid: torch.Tensor, norm, layer_scale: torch.Tensor, *, post_norm=None, next_norm=None):
     """``mid + gamma * out_proj(norm(mid))`` -- the tail of the reference's Mamba block (``model.py:258-260``)
-    as one normalisation kernel and one layer call whose epilogue adds the scaled result to ``mid``."""
-    return out_proj.forward_fused(mid, pre_norm=norm, residual=mid, layer_scale=layer_scale)
+    as one normalisation kernel and one layer call whose epilogue adds the scaled result to ``mid``.  ``post_norm`` (on the
+    layer's output) and ``next_norm`` (the next block's, returned beside the sum) as in ``forward_fused``."""
+    return out_proj.forward_fused(mid, pre_norm=norm, residual=mid, layer_scale=layer_scale, post_norm=post_norm, next_norm=next_norm)
 
 
 def _gate_up_one_launch(ffn_gate: TuckerMoE, ffn_up: TuckerMoE, x: torch.Tensor, norm_w: torch.Tensor, norm_eps: float):
@@ -735,16 +786,17 @@ def _gate_up_one_launch(ffn_gate: TuckerMoE, ffn_up: TuckerMoE, x: torch.Tensor,
 
 
 def fused_ffn(ffn_gate: TuckerMoE, ffn_up: TuckerMoE, ffn_down: TuckerMoE, x_res: torch.Tensor, norm,
-              layer_scale: torch.Tensor) -> torch.Tensor:
+              layer_scale: torch.Tensor, *, post_norm=None, next_norm=None):
     """``x_res + gamma * ffn_down(silu(ffn_gate(x_f)) * ffn_up(x_f))`` with ``x_f = norm(x_res)`` -- the FFN of the
     reference's transformer block (``model.py:337-341``).  The norm runs inside the gate and up layers' in-projection kernels where those
     support it (else ``x_f`` is computed once and shared); on the tensor-core path the two layers' in-projection / core stages are one
     launch that reads each tile of ``x_res`` from HBM once, ``silu(gate) * up`` is the epilogue of the up layer and the residual add is the epilogue of the down
-    layer, so no element-wise pass over the 6x-wide activations remains."""
+    layer, so no element-wise pass over the 6x-wide activations remains.  ``post_norm`` (on ffn_down's output) and ``next_norm`` (the next
+    block's, returned beside the sum) as in ``forward_fused``."""
     w, e = (norm.weight, norm.eps) if hasattr(norm, "weight") else norm
     act = _gate_up_one_launch(ffn_gate, ffn_up, x_res, w, e)
     if act is not None:
-        return ffn_down.forward_fused(act, residual=x_res, layer_scale=layer_scale)
+        return ffn_down.forward_fused(act, residual=x_res, layer_scale=layer_scale, post_norm=post_norm, next_norm=next_norm)
     if ffn_gate._prepared_prenorm_for(x_res, w) is not None and ffn_up._prepared_prenorm_for(x_res, w) is not None:
         # both layers apply the norm inside their in-projection kernels: no separate pass over x_res
         gate = ffn_gate.forward_fused(x_res, pre_norm=(w, e))
@@ -753,4 +805,4 @@ def fused_ffn(ffn_gate: TuckerMoE, ffn_up: TuckerMoE, ffn_down: TuckerMoE, x_res
         x_f = rms_norm(x_res, w, e)
         gate = ffn_gate(x_f)
         act = ffn_up.forward_fused(x_f, silu_gate=gate)
-    return ffn_down.forward_fused(act, residual=x_res, layer_scale=layer_scale)
+    return ffn_down.forward_fused(act, residual=x_res, layer_scale=layer_scale, post_norm=post_norm, next_norm=next_norm)
