@@ -30,8 +30,10 @@
 namespace tmoe {
 namespace {
 
-constexpr int kRouteThreads = 256;
+constexpr int kRouteThreads = 256;                       // backward
 constexpr int kRouteWarps = kRouteThreads / 32;
+// Forward: 512 where a lane holds 8 columns, so that fewer blocks leave partial rows; 256 where it holds more
+constexpr int forward_threads(int NC) { return NC == 1 ? 512 : 256; }
 constexpr int kRouteMaxExperts = 1024;
 
 struct RouteArgs {
@@ -58,8 +60,8 @@ struct RouteArgs {
 template <typename TS> struct Key;
 template <> struct Key<bf16> {
   using type = uint32_t;   // order-preserving bits of the score << 16 | 0xffff - column
-  // the keys of 8 scores, two to a word, in columns col .. col + 7
-  __device__ static __forceinline__ void make(const uint4 &v, int col, uint32_t (&key)[8]) {
+  // the keys of 8 scores, two to a word; low[i] = 0xffff - column of score i
+  __device__ static __forceinline__ void make(const uint4 &v, const uint32_t (&low)[8], uint32_t (&key)[8]) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -68,8 +70,8 @@ template <> struct Key<bf16> {
       uint32_t neg;                                            // 0xffff in the halves whose sign is set
       asm("prmt.b32 %0, %1, 0, 0xbb99;" : "=r"(neg) : "r"(u));
       const uint32_t o = u ^ (neg | 0x80008000u);
-      key[2 * i] = (o << 16) + (0xffffu - (uint32_t)(col + 2 * i));
-      key[2 * i + 1] = (o & 0xffff0000u) + (0xffffu - (uint32_t)(col + 2 * i + 1));
+      asm("mad.lo.u32 %0, %1, 65536, %2;" : "=r"(key[2 * i]) : "r"(o), "r"(low[2 * i]));
+      key[2 * i + 1] = (o & 0xffff0000u) | low[2 * i + 1];
     }
   }
   __device__ static __forceinline__ bool empty(uint32_t key) { return (key >> 16) <= 0x7fu; }
@@ -93,6 +95,9 @@ template <> struct Key<float> {
     return __uint_as_float((u & 0x80000000u) ? (u & 0x7fffffffu) : ~u);
   }
 };
+
+// 4 keys of bf16 scores or 2 of fp32 ones behind a list keep its rows 16-byte aligned
+template <typename TS> struct Lists { static constexpr int kPad = sizeof(TS) == 2 ? 4 : 2; };
 
 // Slots that one lane of a token's G lanes keeps: slot j lives in lane j % G.  k is at most 16 and at most E <= 8 * G here.
 template <int G> struct Slots { static constexpr int N = G <= 2 ? 8 : G == 4 ? 4 : G == 8 ? 2 : 1; };
@@ -138,7 +143,7 @@ template <bool WIDE> struct Chunk<bf16, WIDE> {
       v = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
     }
   }
-  __device__ __forceinline__ void keys(int e0, uint32_t (&key)[8]) const { Key<bf16>::make(v, e0, key); }
+  __device__ __forceinline__ void keys(int, const uint32_t (&low)[8], uint32_t (&key)[8]) const { Key<bf16>::make(v, low, key); }
   __device__ __forceinline__ f2 get(int j) const {
     const uint32_t w = j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w;
     return pair(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
@@ -160,7 +165,7 @@ template <bool WIDE> struct Chunk<float, WIDE> {
         if (e0 + q < E) v[q] = row[e0 + q];
     }
   }
-  __device__ __forceinline__ void keys(int e0, unsigned long long (&key)[8]) const {
+  __device__ __forceinline__ void keys(int e0, const uint32_t (&)[8], unsigned long long (&key)[8]) const {
 #pragma unroll
     for (int q = 0; q < 8; ++q) key[q] = Key<float>::one(v[q], e0 + q);
   }
@@ -170,24 +175,24 @@ template <bool WIDE> struct Chunk<float, WIDE> {
 // Capped, tempered logits l = scale * tanh(v * inv_cap) of N values and, for GRAD, their derivatives.  tanh up to 1 in magnitude is the Pade
 // approximant x (945 + 105 x^2 + x^4) / (945 + 420 x^2 + 15 x^4) that Lambert's continued fraction gives (6e-8 off at 1, less below) with
 // derivative 1 - t^2.  Beyond that, where 1 - t^2 cancels, both come from e = exp(-2|x|), and a score of -inf, which the cap would make a number
-// again, is put back to -inf.  That second part is skipped unless a lane of the warp needs it: scores seldom reach the cap.  NaN stays NaN.
+// again, is put back to -inf.  That second part is skipped unless a lane of the warp may need it, told by the sum of its x^2 (paired FMAs;
+// compares would go to the pipe that the selection fills): scores seldom reach the cap.  NaN stays NaN.
 template <int N2, bool GRAD>
 __device__ __forceinline__ void cap_logits(const RouteArgs &a, f2 (&l)[N2], f2 (&d)[GRAD ? N2 : 1]) {
   f2 x[N2];
-  bool far = false;
+  f2 all = both(0.f);
 #pragma unroll
   for (int j = 0; j < N2; ++j) {
     x[j] = mul2(l[j], both(a.inv_cap));
-    float xa, xb, da, db;
-    split(x[j], xa, xb);
-    far = far || fabsf(xa) > 1.f || fabsf(xb) > 1.f;
+    float da, db;
     const f2 q = mul2(x[j], x[j]);
+    all = add2(all, q);
     split(fma2(q, fma2(q, both(15.f), both(420.f)), both(945.f)), da, db);
     const f2 t = mul2(mul2(x[j], fma2(q, add2(q, both(105.f)), both(945.f))), pair(fast_rcp(da), fast_rcp(db)));
     l[j] = mul2(t, both(a.scale));
     if (GRAD) d[j] = mul2(fma2(mul2(t, both(-1.f)), t, both(1.f)), both(a.scale * a.inv_cap));
   }
-  if (!__any_sync(0xffffffffu, far)) return;
+  if (!__any_sync(0xffffffffu, !(sum2(all) <= 1.f))) return;
 #pragma unroll
   for (int j = 0; j < N2; ++j) {
     float v[2], lj[2], dj[2] = {0.f, 0.f};
@@ -247,24 +252,36 @@ __device__ __forceinline__ void write_losses(const RouteArgs &a, float dot, floa
 
 // G lanes per token, 8 columns of NC chunks each; a warp walks over tokens with all its groups, and every lane owns the same columns in all
 // of them, so P is a sum in its registers; the choices are counted in shared memory (integers: the order of the atomics does not matter).
-// A lane's keys are sorted once, so that a round of the selection is one maximum over the lanes' heads and a shift in the winner's list.
+// A lane sorts its keys once and leaves them in shared memory, so that a round of the selection is one maximum over the lanes' heads and one
+// load by the winner (shifting the list in registers instead kept the integer pipe busy for two thirds of the kernel).
 // Blocks write one row of partial sums each; a block that is alone finishes the losses itself.
 template <typename TS, int G, int NC, int DEPTH, bool WIDE>
-__global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_constant__ RouteArgs a) {
+__global__ void __launch_bounds__(forward_threads(NC)) route_kernel(const __grid_constant__ RouteArgs a) {
   using K = Key<TS>;
+  constexpr int THREADS = forward_threads(NC), WARPS = THREADS / 32;
   constexpr int N = NC * 8, SL = Slots<G>::N, PER = 32 / G;   // columns and slots per lane, tokens per warp
-  extern __shared__ float sm[];                               // [warps][G * N]
+  extern __shared__ __align__(16) float sm[];                 // the lanes' lists; after the walk [warps][G * N] sums
   __shared__ int hist[G * N];
+  // a lane's NC lists of DEPTH keys, each with a 0 behind it (an exhausted list; equal to no chosen key but an exhausted row's), 16-byte rows
+  constexpr int kPad = Lists<TS>::kPad;
+  typename K::type *list = reinterpret_cast<typename K::type *>(sm) + (size_t)threadIdx.x * NC * (DEPTH + kPad);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gl = lane % G, grp = lane / G;
   ptx::griddep_launch_dependents();
-  for (int i = threadIdx.x; i < G * N; i += kRouteThreads) hist[i] = 0;
+  for (int i = threadIdx.x; i < G * N; i += THREADS) hist[i] = 0;
   __syncthreads();
   f2 acc[N / 2];
 #pragma unroll
   for (int x = 0; x < N / 2; ++x) acc[x] = both(0.f);
   float zsum = 0.f, nsum = 0.f;
-  const int64_t step = (int64_t)gridDim.x * kRouteWarps * PER;
-  int64_t t = ((int64_t)blockIdx.x * kRouteWarps + warp) * PER + grp;
+  uint32_t low[NC][8];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    list[c * (DEPTH + kPad) + DEPTH] = 0;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) low[c][q] = 0xffffu - (uint32_t)((c * G + gl) * 8 + q);
+  }
+  const int64_t step = (int64_t)gridDim.x * WARPS * PER;
+  int64_t t = ((int64_t)blockIdx.x * WARPS + warp) * PER + grp;
   Chunk<TS, WIDE> next[NC];                                   // one token ahead
   auto fetch = [&](int64_t at) {
     const bool want = at < a.tokens && (!a.mask || a.mask[at]);
@@ -275,35 +292,37 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_const
   for (; t - grp < a.tokens; t += step) {
     const bool here = t < a.tokens;
     Chunk<TS, WIDE> s[NC];
-    typename K::type key[NC][8];
+    typename K::type head[NC], mine[SL], first = 0;
+    const typename K::type *at[NC];
 #pragma unroll
     for (int c = 0; c < NC; ++c) s[c] = next[c];
     fetch(t + step);
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      s[c].keys((c * G + gl) * 8, key[c]);
-      sort_keys<DEPTH>(key[c]);
+      typename K::type key[8];
+      s[c].keys((c * G + gl) * 8, low[c], key);
+      sort_keys<DEPTH>(key);
+      typename K::type *to = list + c * (DEPTH + kPad);
+#pragma unroll
+      for (int q = 0; q < DEPTH; ++q) to[q] = key[q];
+      head[c] = key[0];
+      at[c] = to;
     }
-    typename K::type mine[SL], first = 0;
 #pragma unroll
     for (int i = 0; i < SL; ++i) {
       mine[i] = 0;
       const int last = min(G, a.k - i * G);
-#pragma unroll 1
+#pragma unroll 4
       for (int jj = 0; jj < last; ++jj) {
-        typename K::type m = key[0][0];
+        typename K::type m = head[0];
 #pragma unroll
-        for (int c = 1; c < NC; ++c) m = key[c][0] > m ? key[c][0] : m;
+        for (int c = 1; c < NC; ++c) m = head[c] > m ? head[c] : m;
         m = group_max<G>(m);
         if (i == 0 && jj == 0) first = m;
         if (gl == jj) mine[i] = m;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          const bool won = key[c][0] == m;
-#pragma unroll
-          for (int q = 0; q + 1 < DEPTH; ++q) key[c][q] = won ? key[c][q + 1] : key[c][q];
-          key[c][DEPTH - 1] = won ? 0 : key[c][DEPTH - 1];
-        }
+        for (int c = 0; c < NC; ++c)
+          if (head[c] == m) head[c] = *++at[c];
       }
     }
     const bool live = !K::empty(first);
@@ -363,6 +382,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_const
       }
     }
   }
+  __syncthreads();   // the lists' memory is reused
   // the block's sums: groups of a warp by shuffles, then the warps in order
 #pragma unroll
   for (int x = 0; x < N; ++x) {
@@ -373,16 +393,16 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_const
     for (int o = G; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if (grp == 0) sm[warp * (G * N) + ((x / 8) * G + gl) * 8 + x % 8] = v;
   }
-  __shared__ float szn[kRouteWarps][3];
+  __shared__ float szn[WARPS][3];
   zsum = warp_sum(zsum); nsum = warp_sum(nsum);
   if (lane == 0) { szn[warp][0] = zsum; szn[warp][1] = nsum; }
   __syncthreads();
   const bool alone = gridDim.x == 1;
   float dot = 0.f;
-  for (int e = threadIdx.x; e < a.E; e += kRouteThreads) {
+  for (int e = threadIdx.x; e < a.E; e += THREADS) {
     float p = 0.f;
 #pragma unroll
-    for (int w = 0; w < kRouteWarps; ++w) p += sm[w * (G * N) + e];
+    for (int w = 0; w < WARPS; ++w) p += sm[w * (G * N) + e];
     if (alone) {
       a.counts[e] = hist[e];
       dot = fmaf((float)hist[e], p, dot);
@@ -399,7 +419,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_const
   if (threadIdx.x == 0) {
     float z = 0.f, n = 0.f, d = 0.f;
 #pragma unroll
-    for (int w = 0; w < kRouteWarps; ++w) { z += szn[w][0]; n += szn[w][1]; d += alone ? szn[w][2] : 0.f; }
+    for (int w = 0; w < WARPS; ++w) { z += szn[w][0]; n += szn[w][1]; d += alone ? szn[w][2] : 0.f; }
     if (alone) {
       write_losses(a, d, z, n);
     } else {
@@ -479,7 +499,7 @@ __global__ void __launch_bounds__(kLossThreads) route_losses_kernel(const __grid
 // p comes from the kept largest logit and sum, so a token needs one pass over its row.  The gates' parts of the gradient go through a row of shared memory
 // per token: the lanes that hold slots put them at their columns, and every lane picks up its own eight.
 template <typename TS, int G, int NC, bool WIDE>
-__global__ void __launch_bounds__(kRouteThreads) route_backward_kernel(const __grid_constant__ RouteArgs a) {
+__global__ void __launch_bounds__(kRouteThreads, NC == 1 && G >= 16 ? 3 : 1) route_backward_kernel(const __grid_constant__ RouteArgs a) {
   constexpr int N = NC * 8, SL = Slots<G>::N, PER = 32 / G;
   extern __shared__ __align__(16) float sm[];   // [warps][PER][G * N]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gl = lane % G, grp = lane / G;
@@ -614,8 +634,8 @@ int lanes_per_token(int E) {
   return g;
 }
 int route_blocks(int64_t tokens, int E, int sms) {
-  const int64_t per = kRouteWarps * (32 / lanes_per_token(E));
-  const int64_t want = (tokens + per - 1) / per, cap = (int64_t)sms * 4;
+  const int64_t per = forward_threads((E + 255) / 256) / 32 * (32 / lanes_per_token(E));
+  const int64_t want = (tokens + per - 1) / per, cap = (int64_t)sms * 2;
   return (int)(want < cap ? want : cap);
 }
 
@@ -664,11 +684,26 @@ bool route_wide(const tmoe_route_t &p, const void *d_scores) {
     else CALL(TS, 32, 4, W);                     \
   } while (0)
 
+template <typename TS, int G, int NC, int DEPTH, bool WIDE>
+void launch_route_as(const RouteArgs &a, int blocks, cudaStream_t st) {
+  constexpr int threads = forward_threads(NC);
+  constexpr int lists = threads * NC * (DEPTH + Lists<TS>::kPad) * (int)sizeof(typename Key<TS>::type), sums = threads / 32 * G * NC * 8 * 4;
+  constexpr int smem = lists > sums ? lists : sums;
+  if (smem > 40 * 1024) {   // (with the static part above what needs no declaration)
+    static std::atomic<uint64_t> opted{0};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (!(opted.load(std::memory_order_relaxed) & bit)) {
+      cudaFuncSetAttribute(route_kernel<TS, G, NC, DEPTH, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+      opted.fetch_or(bit, std::memory_order_relaxed);
+    }
+  }
+  route_kernel<TS, G, NC, DEPTH, WIDE><<<blocks, threads, smem, st>>>(a);
+}
 template <typename TS>
 void launch_route(const RouteArgs &a, bool wide, int blocks, cudaStream_t st) {
-#define TMOE_RT(TS_, G, NC, W)                                                                                          \
-  (a.k <= 2 ? (void)route_kernel<TS_, G, NC, 2, W><<<blocks, kRouteThreads, kRouteWarps * G * NC * 8 * 4, st>>>(a)      \
-            : (void)route_kernel<TS_, G, NC, 8, W><<<blocks, kRouteThreads, kRouteWarps * G * NC * 8 * 4, st>>>(a))
+#define TMOE_RT(TS_, G, NC, W) (a.k <= 2 ? launch_route_as<TS_, G, NC, 2, W>(a, blocks, st) : launch_route_as<TS_, G, NC, 8, W>(a, blocks, st))
   if (wide) TMOE_ROUTE_G(TMOE_RT, TS, true);
   else TMOE_ROUTE_G(TMOE_RT, TS, false);
 #undef TMOE_RT
@@ -759,7 +794,7 @@ int tmoe_route_tokens_backward(const tmoe_route_t *p, const int32_t *idx, const 
   a.d_gates = d_gates; a.d_balance = d_balance; a.d_z = d_z; a.d_scores = d_scores;
   const bool wide = route_wide(*p, d_scores);
   const int64_t per = kRouteWarps * (32 / lanes_per_token(a.E)), want = (a.tokens + per - 1) / per;
-  const int blocks = (int)(want < (int64_t)sms * 8 ? want : (int64_t)sms * 8);
+  const int blocks = (int)(want < (int64_t)sms * 3 ? want : (int64_t)sms * 3);
   cudaStream_t st = (cudaStream_t)stream;
   if (p->dtype == TMOE_F32) launch_route_backward<float>(a, wide, blocks, st);
   else launch_route_backward<bf16>(a, wide, blocks, st);
