@@ -75,6 +75,8 @@ template <int KV> struct SlotPack {
 // One thread makes C neighbouring coefficients of a token; the U_expert table comes from L1.
 template <typename TU, int C, int KV>
 __global__ void __launch_bounds__(256) coef_kernel(const __grid_constant__ CoefArgs a) {
+  ptx::griddep_launch_dependents();
+  ptx::griddep_wait();   // the routing may come from the kernel before this one
   const int per = a.r1 / C;
   const int64_t n = a.T * per;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
@@ -104,6 +106,8 @@ __global__ void __launch_bounds__(256) coef_kernel(const __grid_constant__ CoefA
 // One thread makes KV neighbouring slots of a token.
 template <typename TU, int C, int KV>
 __global__ void __launch_bounds__(256) coef_d_gates_kernel(const __grid_constant__ CoefArgs a) {
+  // in this order: once the next kernel may start, what was before this one is complete (coef_d_u_kernel counts on it)
+  ptx::griddep_wait();
   ptx::griddep_launch_dependents();
   const int per = a.k / KV;
   const int64_t n = a.T * per;
@@ -310,18 +314,22 @@ int spread(int64_t threads, int sms) {
   return (int)(want < cap ? want : cap);
 }
 template <typename TU, int C>
-void launch_coef(const CoefArgs &a, int sms, cudaStream_t st) {
+int launch_coef(const CoefArgs &a, int sms, cudaStream_t st) {
   const int blocks = spread(a.T * (a.r1 / C), sms), kv = slots_wide(a);
-  if (kv == 4) coef_kernel<TU, C, 4><<<blocks, 256, 0, st>>>(a);
-  else if (kv == 2) coef_kernel<TU, C, 2><<<blocks, 256, 0, st>>>(a);
-  else coef_kernel<TU, C, 1><<<blocks, 256, 0, st>>>(a);
+  const dim3 grid((unsigned)blocks), block(256);
+  count_launch();
+  return cuda_ok(kv == 4   ? launch_pdl(coef_kernel<TU, C, 4>, grid, block, 0, st, a)
+                 : kv == 2 ? launch_pdl(coef_kernel<TU, C, 2>, grid, block, 0, st, a)
+                           : launch_pdl(coef_kernel<TU, C, 1>, grid, block, 0, st, a));
 }
 template <typename TU, int C>
-void launch_d_gates(const CoefArgs &a, int sms, cudaStream_t st) {
+int launch_d_gates(const CoefArgs &a, int sms, cudaStream_t st) {
   const int kv = slots_wide(a), blocks = spread(a.T * (a.k / kv), sms);
-  if (kv == 4) coef_d_gates_kernel<TU, C, 4><<<blocks, 256, 0, st>>>(a);
-  else if (kv == 2) coef_d_gates_kernel<TU, C, 2><<<blocks, 256, 0, st>>>(a);
-  else coef_d_gates_kernel<TU, C, 1><<<blocks, 256, 0, st>>>(a);
+  const dim3 grid((unsigned)blocks), block(256);
+  count_launch();
+  return cuda_ok(kv == 4   ? launch_pdl(coef_d_gates_kernel<TU, C, 4>, grid, block, 0, st, a)
+                 : kv == 2 ? launch_pdl(coef_d_gates_kernel<TU, C, 2>, grid, block, 0, st, a)
+                           : launch_pdl(coef_d_gates_kernel<TU, C, 1>, grid, block, 0, st, a));
 }
 
 }  // namespace
@@ -343,10 +351,8 @@ int tmoe_expert_coef(const tmoe_expert_coef_t *p, float *c, void *stream) {
   a.c = c;
   const bool four = cols_by_4(a, p->dtype == TMOE_F32 ? 4 : 2, c);
   cudaStream_t st = (cudaStream_t)stream;
-  if (p->dtype == TMOE_F32) four ? launch_coef<float, 4>(a, sms, st) : launch_coef<float, 1>(a, sms, st);
-  else four ? launch_coef<bf16, 4>(a, sms, st) : launch_coef<bf16, 1>(a, sms, st);
-  count_launch();
-  return launch_status();
+  if (p->dtype == TMOE_F32) return four ? launch_coef<float, 4>(a, sms, st) : launch_coef<float, 1>(a, sms, st);
+  return four ? launch_coef<bf16, 4>(a, sms, st) : launch_coef<bf16, 1>(a, sms, st);
 }
 
 int64_t tmoe_expert_coef_workspace_bytes(const tmoe_expert_coef_t *p) {
@@ -374,10 +380,9 @@ int tmoe_expert_coef_backward(const tmoe_expert_coef_t *p, const float *d_c, flo
   a.d_c = d_c; a.d_gates = d_gates;
   if (d_gates) {
     const bool four = cols_by_4(a, size, d_c);
-    if (p->dtype == TMOE_F32) four ? launch_d_gates<float, 4>(a, sms, st) : launch_d_gates<float, 1>(a, sms, st);
-    else four ? launch_d_gates<bf16, 4>(a, sms, st) : launch_d_gates<bf16, 1>(a, sms, st);
-    count_launch();
-    if ((rc = launch_status())) return rc;
+    if (p->dtype == TMOE_F32) rc = four ? launch_d_gates<float, 4>(a, sms, st) : launch_d_gates<float, 1>(a, sms, st);
+    else rc = four ? launch_d_gates<bf16, 4>(a, sms, st) : launch_d_gates<bf16, 1>(a, sms, st);
+    if (rc) return rc;
   }
   if (d_U_expert) {
     const DuShape s = du_shape(a.T, a.E, a.k, a.r1, sms < 160 ? sms : 160);

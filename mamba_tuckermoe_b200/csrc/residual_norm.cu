@@ -357,7 +357,9 @@ template <typename TY, typename TR, int VEC, int NV, bool GATE>
 __global__ void __launch_bounds__(512, VEC == 8 && NV == 1 ? 2 : 1) residual_norm_kernel(const __grid_constant__ NormArgs a) {
   using In = RowIn<TY, TR, VEC, NV, GATE, false>;
   __shared__ __align__(16) TeamRed<1> red;
+  ptx::griddep_launch_dependents();
   red.init();
+  ptx::griddep_wait();   // the operands may come from the kernel before this one
   const int tpr = a.tw * 32, team = threadIdx.x / tpr, lt = threadIdx.x - team * tpr;
   int row = blockIdx.x * (blockDim.x / tpr) + team;
   int64_t off = (int64_t)row * a.d;     // of the row in the outputs
@@ -408,6 +410,7 @@ __global__ void __launch_bounds__(32 * block_warps(VEC == 8 ? NV : NV / 8, true,
   __shared__ __align__(16) TeamRed<3> red;
   ptx::griddep_launch_dependents();
   red.init();
+  ptx::griddep_wait();
   const int tpr = a.tw * 32, team = threadIdx.x / tpr, lt = threadIdx.x - team * tpr, teams = blockDim.x / tpr;
   int row = blockIdx.x * teams + team;
   int64_t off = (int64_t)row * a.d;     // of the row in the outputs
@@ -611,13 +614,13 @@ bool norm_wide(const tmoe_residual_norm_t &p) {
 // Launch with the ring's shared memory; its size (and that the SM should be split for it: without that fewer blocks are resident
 // than the grid counts on) is declared once per kernel and device
 template <typename In, typename Kernel>
-void launch_walk(Kernel kernel, const NormArgs &a, const NormShape &s, bool fold, cudaStream_t st) {
+int launch_walk(Kernel kernel, const NormArgs &a, const NormShape &s, bool fold, cudaStream_t st) {
   static std::atomic<uint64_t> opted{0};
   const int threads = s.teams * s.tw * 32;
   size_t smem = In::kRing ? (size_t)(In::kStages * In::kPlanes + In::kParamPlanes) * threads * 16 : 0;
   if (fold && s.teams > 1 && smem < (size_t)a.d * 4) smem = (size_t)a.d * 4;
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return;
+  if (cudaGetDevice(&dev) != cudaSuccess) return TMOE_ERR_CUDA;
   const uint64_t bit = 1ull << (dev & 63);
   if (In::kRing && !(opted.load(std::memory_order_relaxed) & bit)) {
     cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
@@ -628,39 +631,31 @@ void launch_walk(Kernel kernel, const NormArgs &a, const NormShape &s, bool fold
   b.step = s.blocks * s.teams;
   b.y_step = b.step * a.ys; b.r_step = b.step * a.rs; b.g_step = b.step * a.gs; b.do_step = b.step * a.dos; b.dn_step = b.step * a.dns;
   b.o_step = (int64_t)b.step * a.d;
-  kernel<<<s.blocks, threads, smem, st>>>(b);
+  count_launch();
+  return cuda_ok(launch_pdl(kernel, dim3((unsigned)s.blocks), dim3((unsigned)threads), smem, st, b));
 }
 
 template <typename TY, typename TR, bool GATE>
-void launch_forward(const NormArgs &a, const NormShape &s, bool wide, cudaStream_t st) {
+int launch_forward(const NormArgs &a, const NormShape &s, bool wide, cudaStream_t st) {
 #define TMOE_RN(V, N) launch_walk<RowIn<TY, TR, V, N, GATE, false>>(residual_norm_kernel<TY, TR, V, N, GATE>, a, s, false, st)
-  if (wide) { if (s.nv == 1) TMOE_RN(8, 1); else TMOE_RN(8, 2); }
-  else { if (s.nv == 1) TMOE_RN(1, 8); else TMOE_RN(1, 16); }
+  if (wide) return s.nv == 1 ? TMOE_RN(8, 1) : TMOE_RN(8, 2);
+  return s.nv == 1 ? TMOE_RN(1, 8) : TMOE_RN(1, 16);
 #undef TMOE_RN
 }
 
 template <typename TY, typename TR, bool GATE>
-void launch_backward(const NormArgs &a, const NormShape &s, bool wide, cudaStream_t st) {
+int launch_backward(const NormArgs &a, const NormShape &s, bool wide, cudaStream_t st) {
 #define TMOE_RNB(V, N) launch_walk<RowIn<TY, TR, V, N, GATE, true>>(residual_norm_backward_kernel<TY, TR, V, N, GATE>, a, s, true, st)
-  if (wide) { if (s.nv == 1) TMOE_RNB(8, 1); else TMOE_RNB(8, 2); }
-  else { if (s.nv == 1) TMOE_RNB(1, 8); else TMOE_RNB(1, 16); }
+  if (wide) return s.nv == 1 ? TMOE_RNB(8, 1) : TMOE_RNB(8, 2);
+  return s.nv == 1 ? TMOE_RNB(1, 8) : TMOE_RNB(1, 16);
 #undef TMOE_RNB
 }
 
 // CALL<y type, residual type, gate>(...) for the call's types
-#define TMOE_NORM_TYPES(CALL, p, ...)                                              \
-  do {                                                                             \
-    if ((p)->dtype == TMOE_F32) {                                                  \
-      if ((p)->gate) CALL<float, float, true>(__VA_ARGS__);                        \
-      else CALL<float, float, false>(__VA_ARGS__);                                 \
-    } else if ((p)->residual_dtype == TMOE_F32) {                                  \
-      if ((p)->gate) CALL<bf16, float, true>(__VA_ARGS__);                         \
-      else CALL<bf16, float, false>(__VA_ARGS__);                                  \
-    } else {                                                                       \
-      if ((p)->gate) CALL<bf16, bf16, true>(__VA_ARGS__);                          \
-      else CALL<bf16, bf16, false>(__VA_ARGS__);                                   \
-    }                                                                              \
-  } while (0)
+#define TMOE_NORM_TYPES(CALL, p, ...)                                                                                              \
+  ((p)->dtype == TMOE_F32 ? ((p)->gate ? CALL<float, float, true>(__VA_ARGS__) : CALL<float, float, false>(__VA_ARGS__))           \
+   : (p)->residual_dtype == TMOE_F32 ? ((p)->gate ? CALL<bf16, float, true>(__VA_ARGS__) : CALL<bf16, float, false>(__VA_ARGS__))  \
+                                     : ((p)->gate ? CALL<bf16, bf16, true>(__VA_ARGS__) : CALL<bf16, bf16, false>(__VA_ARGS__)))
 
 }  // namespace
 }  // namespace tmoe
@@ -685,9 +680,7 @@ int tmoe_residual_norm(const tmoe_residual_norm_t *p, void *out, void *normed, f
   if (sms <= 0) return TMOE_ERR_CUDA;
   const NormShape s = norm_shape(*p, false, sms);
   a.tw = s.tw;
-  TMOE_NORM_TYPES(launch_forward, p, a, s, wide, st);
-  count_launch();
-  return launch_status();
+  return TMOE_NORM_TYPES(launch_forward, p, a, s, wide, st);
 }
 
 int64_t tmoe_residual_norm_workspace_bytes(const tmoe_residual_norm_t *p) {
@@ -739,9 +732,7 @@ int tmoe_residual_norm_backward(const tmoe_residual_norm_t *p, const float *rstd
   const bool wide = norm_wide(*p) && wide_ok(d_out, d_out_stride, sr) && wide_ok(d_normed, d_normed_stride, sy) &&
                     wide_ok(d_y, p->d, sy) && wide_ok(d_residual, p->d, sr) && wide_ok(d_gate, p->d, sy);
   a.tw = s.tw;
-  TMOE_NORM_TYPES(launch_backward, p, a, s, wide, st);
-  count_launch();
-  if ((rc = launch_status())) return rc;
+  if ((rc = TMOE_NORM_TYPES(launch_backward, p, a, s, wide, st))) return rc;
   if (params) {
     const dim3 grid((unsigned)((a.n_sums * p->d + 31) / 32)), block(kColumnSumThreads);
     if (p->dtype == TMOE_F32)

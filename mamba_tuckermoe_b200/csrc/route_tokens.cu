@@ -269,6 +269,7 @@ __global__ void __launch_bounds__(forward_threads(NC)) route_kernel(const __grid
   ptx::griddep_launch_dependents();
   for (int i = threadIdx.x; i < G * N; i += THREADS) hist[i] = 0;
   __syncthreads();
+  ptx::griddep_wait();   // the scores may come from the kernel before this one
   f2 acc[N / 2];
 #pragma unroll
   for (int x = 0; x < N / 2; ++x) acc[x] = both(0.f);
@@ -504,8 +505,10 @@ __global__ void __launch_bounds__(kRouteThreads, NC == 1 && G >= 16 ? 3 : 1) rou
   extern __shared__ __align__(16) float sm[];   // [warps][PER][G * N]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gl = lane % G, grp = lane / G;
   float *row = sm + (warp * PER + grp) * (G * N);
+  ptx::griddep_launch_dependents();
   for (int i = gl; i < G * N; i += G) row[i] = 0.f;
   __syncwarp();
+  ptx::griddep_wait();
   const float n = a.losses[2], inv_n = n > 0.f ? 1.f / n : 0.f;
   const float z2 = a.d_z ? *a.d_z * 2.f * inv_n : 0.f;
   const float bal = a.d_balance ? *a.d_balance * ((float)a.E * inv_n) * (inv_n / (float)a.k) : 0.f;
@@ -672,47 +675,46 @@ bool route_wide(const tmoe_route_t &p, const void *d_scores) {
 }
 
 // The kernel for E experts: G lanes x NC pieces of 8 columns cover them
-#define TMOE_ROUTE_G(CALL, TS, W)                \
-  do {                                           \
-    if (a.E <= 8) CALL(TS, 1, 1, W);             \
-    else if (a.E <= 16) CALL(TS, 2, 1, W);       \
-    else if (a.E <= 32) CALL(TS, 4, 1, W);       \
-    else if (a.E <= 64) CALL(TS, 8, 1, W);       \
-    else if (a.E <= 128) CALL(TS, 16, 1, W);     \
-    else if (a.E <= 256) CALL(TS, 32, 1, W);     \
-    else if (a.E <= 512) CALL(TS, 32, 2, W);     \
-    else CALL(TS, 32, 4, W);                     \
-  } while (0)
+#define TMOE_ROUTE_G(CALL, TS, W)                              \
+  (a.E <= 8     ? CALL(TS, 1, 1, W)                            \
+   : a.E <= 16  ? CALL(TS, 2, 1, W)                            \
+   : a.E <= 32  ? CALL(TS, 4, 1, W)                            \
+   : a.E <= 64  ? CALL(TS, 8, 1, W)                            \
+   : a.E <= 128 ? CALL(TS, 16, 1, W)                           \
+   : a.E <= 256 ? CALL(TS, 32, 1, W)                           \
+   : a.E <= 512 ? CALL(TS, 32, 2, W)                           \
+                : CALL(TS, 32, 4, W))
 
 template <typename TS, int G, int NC, int DEPTH, bool WIDE>
-void launch_route_as(const RouteArgs &a, int blocks, cudaStream_t st) {
+int launch_route_as(const RouteArgs &a, int blocks, cudaStream_t st) {
   constexpr int threads = forward_threads(NC);
   constexpr int lists = threads * NC * (DEPTH + Lists<TS>::kPad) * (int)sizeof(typename Key<TS>::type), sums = threads / 32 * G * NC * 8 * 4;
   constexpr int smem = lists > sums ? lists : sums;
   if (smem > 40 * 1024) {   // (with the static part above what needs no declaration)
     static std::atomic<uint64_t> opted{0};
     int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return;
+    if (cudaGetDevice(&dev) != cudaSuccess) return TMOE_ERR_CUDA;
     const uint64_t bit = 1ull << (dev & 63);
     if (!(opted.load(std::memory_order_relaxed) & bit)) {
       cudaFuncSetAttribute(route_kernel<TS, G, NC, DEPTH, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
       opted.fetch_or(bit, std::memory_order_relaxed);
     }
   }
-  route_kernel<TS, G, NC, DEPTH, WIDE><<<blocks, threads, smem, st>>>(a);
+  count_launch();
+  return cuda_ok(launch_pdl(route_kernel<TS, G, NC, DEPTH, WIDE>, dim3((unsigned)blocks), dim3(threads), smem, st, a));
 }
 template <typename TS>
-void launch_route(const RouteArgs &a, bool wide, int blocks, cudaStream_t st) {
+int launch_route(const RouteArgs &a, bool wide, int blocks, cudaStream_t st) {
 #define TMOE_RT(TS_, G, NC, W) (a.k <= 2 ? launch_route_as<TS_, G, NC, 2, W>(a, blocks, st) : launch_route_as<TS_, G, NC, 8, W>(a, blocks, st))
-  if (wide) TMOE_ROUTE_G(TMOE_RT, TS, true);
-  else TMOE_ROUTE_G(TMOE_RT, TS, false);
+  return wide ? TMOE_ROUTE_G(TMOE_RT, TS, true) : TMOE_ROUTE_G(TMOE_RT, TS, false);
 #undef TMOE_RT
 }
 template <typename TS>
-void launch_route_backward(const RouteArgs &a, bool wide, int blocks, cudaStream_t st) {
-#define TMOE_RTB(TS_, G, NC, W) route_backward_kernel<TS_, G, NC, W><<<blocks, kRouteThreads, kRouteWarps * 32 * NC * 8 * 4, st>>>(a)
-  if (wide) TMOE_ROUTE_G(TMOE_RTB, TS, true);
-  else TMOE_ROUTE_G(TMOE_RTB, TS, false);
+int launch_route_backward(const RouteArgs &a, bool wide, int blocks, cudaStream_t st) {
+#define TMOE_RTB(TS_, G, NC, W) \
+  cuda_ok(launch_pdl(route_backward_kernel<TS_, G, NC, W>, dim3((unsigned)blocks), dim3(kRouteThreads), kRouteWarps * 32 * NC * 8 * 4, st, a))
+  count_launch();
+  return wide ? TMOE_ROUTE_G(TMOE_RTB, TS, true) : TMOE_ROUTE_G(TMOE_RTB, TS, false);
 #undef TMOE_RTB
 }
 
@@ -760,11 +762,8 @@ int tmoe_route_tokens(const tmoe_route_t *p, int32_t *idx, float *gates, int32_t
   a.part_c = reinterpret_cast<int32_t *>(ws + one);
   a.part_zn = reinterpret_cast<float *>(ws + 2 * one);
   const bool wide = route_wide(*p, nullptr);
-  if (p->dtype == TMOE_F32) launch_route<float>(a, wide, blocks, st);
-  else launch_route<bf16>(a, wide, blocks, st);
-  count_launch();
-  if ((rc = launch_status())) return rc;
-  if (blocks == 1) return TMOE_OK;
+  rc = p->dtype == TMOE_F32 ? launch_route<float>(a, wide, blocks, st) : launch_route<bf16>(a, wide, blocks, st);
+  if (rc || blocks == 1) return rc;
   const int per = (a.E + kLossBlocks - 1) / kLossBlocks;
   int width = 1;
   while (width < per && width < 64) width *= 2;
@@ -796,10 +795,7 @@ int tmoe_route_tokens_backward(const tmoe_route_t *p, const int32_t *idx, const 
   const int64_t per = kRouteWarps * (32 / lanes_per_token(a.E)), want = (a.tokens + per - 1) / per;
   const int blocks = (int)(want < (int64_t)sms * 3 ? want : (int64_t)sms * 3);
   cudaStream_t st = (cudaStream_t)stream;
-  if (p->dtype == TMOE_F32) launch_route_backward<float>(a, wide, blocks, st);
-  else launch_route_backward<bf16>(a, wide, blocks, st);
-  count_launch();
-  return launch_status();
+  return p->dtype == TMOE_F32 ? launch_route_backward<float>(a, wide, blocks, st) : launch_route_backward<bf16>(a, wide, blocks, st);
 }
 
 }  // extern "C"
