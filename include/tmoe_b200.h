@@ -264,7 +264,7 @@ typedef struct tmoe_route {
   const void *scores;
   const uint8_t *token_mask; /* [tokens], or NULL: every token counts */
 } tmoe_route_t;
-int64_t tmoe_route_workspace_bytes(const tmoe_route_t *p);   /* of the forward call */
+int64_t tmoe_route_workspace_bytes(const tmoe_route_t *p);   /* of the forward call; 0 for few tokens */
 /* idx, gates [tokens, top_k] (descending score), counts [n_experts], losses [3]; stats [tokens, 2], 8-byte
  * aligned: what the backward call needs of the tokens that count (largest logit, sum of exp(logit - largest)), or NULL */
 int tmoe_route_tokens(const tmoe_route_t *p, int32_t *idx, float *gates, int32_t *counts, float *losses, float *stats, void *workspace,

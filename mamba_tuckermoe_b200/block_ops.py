@@ -152,7 +152,7 @@ def _norm_forward(y, residual, gate, layer_scale, post_w, next_w, post_eps, next
     if next_w is not None:
         normed = _like(y)
     if keep:
-        rstd = _empty((2, p.rows), dtype=_F32, device=device)
+        rstd = y.new_empty((2, p.rows), dtype=_F32)
     _call(device, "tmoe_residual_norm", _lib.load().tmoe_residual_norm, C.byref(p), _ptr(out), _ptr(normed), _ptr(rstd))
     return out, normed, rstd
 
@@ -173,7 +173,7 @@ def _norm_backward(y, residual, gate, layer_scale, post_w, next_w, post_eps, nex
     lib, ws, n = _lib.load(), None, 0
     if want[3] or want[4] or want[5]:
         n = _size("tmoe_residual_norm_workspace_bytes", lib.tmoe_residual_norm_workspace_bytes, p)
-        ws = _empty(n, dtype=_U8, device=device)
+        ws = y.new_empty(n, dtype=_U8)
     _call(device, "tmoe_residual_norm_backward", lib.tmoe_residual_norm_backward, C.byref(p), _ptr(rstd), _ptr(do2), do_stride,
           _ptr(dn2), dn_stride, *[None if g is None else g.data_ptr() for g in grads], _ptr(ws), n)
     return grads
@@ -330,16 +330,16 @@ def _route_forward(scores, mask, top_k, router, keep=False):
     _check_route(scores, top_k, mask)
     p, held = _route_struct(scores, mask, top_k, router)
     slots, dev = (*scores.shape[:-1], top_k), scores.device
-    idx = _empty(slots, dtype=_I32, device=dev)
-    gates = _empty(slots, dtype=_F32, device=dev)
-    counts = _empty(scores.shape[-1], dtype=_I32, device=dev)
-    losses = _empty(3, dtype=_F32, device=dev)
-    stats = _empty((p.tokens, 2), dtype=_F32, device=dev) if keep else None
+    idx = scores.new_empty(slots, dtype=_I32)
+    gates = torch.empty_like(idx, dtype=_F32)
+    counts = scores.new_empty(scores.shape[-1], dtype=_I32)
+    losses = scores.new_empty(3, dtype=_F32)
+    stats = scores.new_empty((p.tokens, 2), dtype=_F32) if keep else None
     lib = _lib.load()
     n = _size("tmoe_route_workspace_bytes", lib.tmoe_route_workspace_bytes, p)
-    ws = _empty(n, dtype=_U8, device=dev)
+    ws = scores.new_empty(n, dtype=_U8) if n else None
     _call(dev, "tmoe_route_tokens", lib.tmoe_route_tokens, C.byref(p), idx.data_ptr(), gates.data_ptr(), counts.data_ptr(),
-          losses.data_ptr(), _ptr(stats), ws.data_ptr(), n)
+          losses.data_ptr(), _ptr(stats), _ptr(ws), n)
     return idx, gates, counts, losses, stats
 
 
@@ -463,7 +463,7 @@ def _coef_struct(idx, gates, u):
 def _coef_forward(idx, gates, u):
     _check_coef(idx, gates, u)
     p, held = _coef_struct(idx, gates, u)
-    c = _empty((*idx.shape[:-1], u.shape[1]), dtype=_F32, device=u.device)
+    c = gates.new_empty((*idx.shape[:-1], u.shape[1]))
     _call(u.device, "tmoe_expert_coef", _lib.load().tmoe_expert_coef, C.byref(p), c.data_ptr())
     return c
 
@@ -476,7 +476,7 @@ def _coef_backward(idx, gates, u, d_c, want_gates, want_u):
     if want_u:
         d_u = _like(u)
         n = _size("tmoe_expert_coef_workspace_bytes", lib.tmoe_expert_coef_workspace_bytes, p)
-        ws = _empty(n, dtype=_U8, device=dev)
+        ws = u.new_empty(n, dtype=_U8)
     _call(dev, "tmoe_expert_coef_backward", lib.tmoe_expert_coef_backward, C.byref(p), d_c.data_ptr(), _ptr(d_gates), _ptr(d_u),
           _ptr(ws), n)
     return d_gates, d_u

@@ -718,7 +718,10 @@ int launch_route_backward(const RouteArgs &a, bool wide, int blocks, cudaStream_
 #undef TMOE_RTB
 }
 
-int64_t route_ws(int blocks, int E) { return align_up((int64_t)blocks * E * 4, 256) * 2 + align_up((int64_t)blocks * 8, 256); }
+// partial rows of the blocks; a block that is alone keeps none
+int64_t route_ws(int blocks, int E) {
+  return blocks == 1 ? 0 : align_up((int64_t)blocks * E * 4, 256) * 2 + align_up((int64_t)blocks * 8, 256);
+}
 
 }  // namespace
 }  // namespace tmoe
@@ -744,7 +747,7 @@ int tmoe_route_tokens(const tmoe_route_t *p, int32_t *idx, float *gates, int32_t
     rc = cuda_ok(cudaMemsetAsync(counts, 0, (size_t)p->n_experts * 4, st));
     return rc ? rc : cuda_ok(cudaMemsetAsync(losses, 0, 12, st));
   }
-  if (!idx || !gates || !workspace) return TMOE_ERR_NULL;
+  if (!idx || !gates) return TMOE_ERR_NULL;
   if ((reinterpret_cast<uintptr_t>(idx) | reinterpret_cast<uintptr_t>(gates) | reinterpret_cast<uintptr_t>(counts) |
        reinterpret_cast<uintptr_t>(losses)) & 3)
     return TMOE_ERR_ALIGN;
@@ -753,7 +756,9 @@ int tmoe_route_tokens(const tmoe_route_t *p, int32_t *idx, float *gates, int32_t
   const int sms = current_device_sms();
   if (sms <= 0) return TMOE_ERR_CUDA;
   const int blocks = route_blocks(p->tokens, p->n_experts, sms < 160 ? sms : 160);
-  if (workspace_bytes < route_ws(blocks, p->n_experts)) return TMOE_ERR_WORKSPACE;
+  const int64_t need = route_ws(blocks, p->n_experts);
+  if (need && !workspace) return TMOE_ERR_NULL;
+  if (workspace_bytes < need) return TMOE_ERR_WORKSPACE;
   RouteArgs a = route_args(*p);
   a.idx = idx; a.gates = gates; a.counts = counts; a.losses = losses; a.stats = stats;
   char *ws = reinterpret_cast<char *>(workspace);
