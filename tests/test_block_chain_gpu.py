@@ -267,3 +267,84 @@ def test_in_place_change_of_a_saved_input_is_noticed():
     res.add_(1.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         normed.sum().backward()
+
+
+def test_rows_beyond_32_bit_offsets():
+    """More than 2^31 elements: the last rows come out as a call on them alone gives them."""
+    d = 8192
+    rows = (1 << 31) // d + 300
+    y = torch.empty(rows, d, dtype=BF, device="cuda")
+    for i in range(0, rows, 1 << 16):
+        y[i:i + (1 << 16)] = torch.arange(i, min(rows, i + (1 << 16)), device="cuda").remainder(97).sub(40).to(BF)[:, None]
+    y[:, ::3] *= 0.5
+    w = torch.linspace(0.5, 1.5, d, device="cuda").to(BF)
+    with torch.no_grad():
+        out, normed = residual_norm(y, layer_scale=w, next_norm=(w, 1e-5))
+        o, n = residual_norm(y[-500:], layer_scale=w, next_norm=(w, 1e-5))
+        assert torch.equal(out[-500:], o) and torch.equal(normed[-500:], n)
+        del out, normed
+        E = 512
+        scores = y.view(-1, E)[: (1 << 31) // E + 1000]
+        r = route_tokens(scores, 2)
+        q = route_tokens(scores[-1500:], 2)
+        assert torch.equal(r.idx[-1500:], q.idx) and torch.equal(r.gates[-1500:], q.gates) and int(r.counts.sum()) == 2 * scores.shape[0]
+    del scores, r
+    leaf = y.requires_grad_()
+    out, _ = residual_norm(leaf, layer_scale=w, post_norm=(w, 1e-5))
+    g, = torch.autograd.grad(out, leaf, y.detach())
+    tail = y.detach()[-300:].clone().requires_grad_()
+    out2, _ = residual_norm(tail, layer_scale=w, post_norm=(w, 1e-5))
+    assert torch.equal(g[-300:], torch.autograd.grad(out2, tail, tail.detach())[0])
+
+
+def test_results_written_over_their_operands():
+    """At the C ABI out may be the residual's buffer and normed y's (dense rows)."""
+    import ctypes as C
+    from mamba_tuckermoe_b200 import _lib
+    lib = _lib.load()
+    for d, dtype in ((768, BF), (1001, F32), (8192, BF)):
+        g = torch.Generator(device="cuda").manual_seed(d)
+        y, res = (torch.randn(3000, d, generator=g, device="cuda").to(dtype) for _ in range(2))
+        w = torch.rand(d, generator=g, device="cuda").to(dtype)
+        want = residual_norm(y, residual=res, post_norm=(w, 1e-5), next_norm=(w, 1e-5))
+        dt = _lib.TMOE_BF16 if dtype == BF else _lib.TMOE_F32
+        p = _lib.ResidualNorm(3000, d, dt, dt, 1e-5, 1e-5, 0, d, d, 0, y.data_ptr(), res.data_ptr(), None, None, w.data_ptr(), w.data_ptr())
+        rc = lib.tmoe_residual_norm(C.byref(p), res.data_ptr(), y.data_ptr(), None, _lib.current_stream_ptr())
+        assert rc == 0 and torch.equal(res, want[0]) and torch.equal(y, want[1])
+
+
+def test_workspace_sizes_are_enough_and_checked():
+    """One byte less than the stated workspace is refused; the stated one is never written beyond."""
+    import ctypes as C
+    from mamba_tuckermoe_b200 import _lib
+    lib, st = _lib.load(), _lib.current_stream_ptr()
+    for rows, d in ((1, 40), (500, 768), (4000, 2304)):
+        y, do = torch.randn(rows, d, device="cuda"), torch.randn(rows, d, device="cuda")
+        w, gw, dy = torch.rand(d, device="cuda"), torch.empty(d, device="cuda"), torch.empty(rows, d, device="cuda")
+        rstd, n_out = torch.empty(2, rows, device="cuda"), torch.empty(rows, d, device="cuda")
+        p = _lib.ResidualNorm(rows, d, 0, 0, 1e-5, 1e-5, 0, d, 0, 0, y.data_ptr(), None, None, None, None, w.data_ptr())
+        assert lib.tmoe_residual_norm(C.byref(p), None, n_out.data_ptr(), rstd.data_ptr(), st) == 0
+        n = lib.tmoe_residual_norm_workspace_bytes(C.byref(p))
+        ws = torch.full((n + 4096,), 171, dtype=torch.uint8, device="cuda")
+        args = lambda size: (C.byref(p), rstd.data_ptr(), None, 0, do.data_ptr(), d, dy.data_ptr(), None, None, None, None, gw.data_ptr(), ws.data_ptr(), size, st)
+        small = lib.tmoe_residual_norm_backward(*args(n // 2 - 1))
+        assert small == -5 and lib.tmoe_residual_norm_backward(*args(n)) == 0
+        assert bool((ws[n:] == 171).all())
+    for T, E, k in ((5000, 64, 2), (700, 1000, 8), (100000, 8, 1)):
+        s = torch.randn(T, E, device="cuda")
+        idx, g = torch.empty(T, k, dtype=torch.int32, device="cuda"), torch.empty(T, k, device="cuda")
+        cnt, loss = torch.empty(E, dtype=torch.int32, device="cuda"), torch.empty(3, device="cuda")
+        p = _lib.Route(T, E, k, 0, 0, 10.0, 0.5, E, s.data_ptr(), None)
+        n = lib.tmoe_route_workspace_bytes(C.byref(p))
+        ws = torch.full((n + 4096,), 171, dtype=torch.uint8, device="cuda")
+        call = lambda size: lib.tmoe_route_tokens(C.byref(p), idx.data_ptr(), g.data_ptr(), cnt.data_ptr(), loss.data_ptr(), None, ws.data_ptr(), size, st)
+        assert call(0) == -5 and call(n) == 0 and bool((ws[n:] == 171).all())
+    for T, E, k, r1 in ((5000, 64, 2, 4), (900, 1024, 8, 64), (40, 8192, 2, 3)):
+        idx = torch.randint(0, E, (T, k), dtype=torch.int32, device="cuda")
+        g, u, dc = torch.rand(T, k, device="cuda"), torch.randn(E, r1, device="cuda"), torch.randn(T, r1, device="cuda")
+        du = torch.empty_like(u)
+        p = _lib.ExpertCoef(T, E, k, r1, 0, idx.data_ptr(), g.data_ptr(), u.data_ptr())
+        n = lib.tmoe_expert_coef_workspace_bytes(C.byref(p))
+        ws = torch.full((n + 4096,), 171, dtype=torch.uint8, device="cuda")
+        call = lambda size: lib.tmoe_expert_coef_backward(C.byref(p), dc.data_ptr(), None, du.data_ptr(), ws.data_ptr(), size, st)
+        assert call(0) == -5 and call(n) == 0 and bool((ws[n:] == 171).all())
