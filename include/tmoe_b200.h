@@ -259,7 +259,8 @@ typedef struct tmoe_route {
   int32_t top_k;           /* 1 .. min(n_experts, TMOE_MAX_TOPK) */
   int32_t dtype;
   int32_t router_mode;     /* tmoe_router_mode_t */
-  float router_cap, router_temperature;
+  float router_cap, router_temperature; /* with TMOE_ROUTER_CAPPED_SOFTMAX > 0, with cap / temperature and both reciprocals
+                              finite and not subnormal */
   int64_t scores_stride;   /* elements between rows */
   const void *scores;
   const uint8_t *token_mask; /* [tokens], or NULL: every token counts */

@@ -172,38 +172,37 @@ template <bool WIDE> struct Chunk<float, WIDE> {
   __device__ __forceinline__ f2 get(int j) const { return pair(v[2 * j], v[2 * j + 1]); }
 };
 
-// Capped, tempered logits l = scale * tanh(v * inv_cap) of N values and, for GRAD, their derivatives.  tanh up to 1 in magnitude is the Pade
+// Capped, tempered logits l = scale * tanh(score * inv_cap) of N2 pairs and, for GRAD, their derivatives.  tanh up to 1 in magnitude is the Pade
 // approximant x (945 + 105 x^2 + x^4) / (945 + 420 x^2 + 15 x^4) that Lambert's continued fraction gives (6e-8 off at 1, less below) with
 // derivative 1 - t^2.  Beyond that, where 1 - t^2 cancels, both come from e = exp(-2|x|), and a score of -inf, which the cap would make a number
-// again, is put back to -inf.  That second part is skipped unless a lane of the warp may need it, told by the sum of its x^2 (paired FMAs;
-// compares would go to the pipe that the selection fills): scores seldom reach the cap.  NaN stays NaN.
-template <int N2, bool GRAD>
-__device__ __forceinline__ void cap_logits(const RouteArgs &a, f2 (&l)[N2], f2 (&d)[GRAD ? N2 : 1]) {
-  f2 x[N2];
+// again, is put back to -inf (the score itself is asked: a finite one over a small cap may overflow, and stays on).  That second part is
+// skipped unless a lane of the warp may need it, told by the sum of its x^2 (paired FMAs; compares would go to the pipe that the selection
+// fills): scores seldom reach the cap.  NaN stays NaN.
+template <int N2, bool GRAD, typename SCORE>
+__device__ __forceinline__ void cap_logits(const RouteArgs &a, const SCORE &score, f2 (&l)[N2], f2 (&d)[GRAD ? N2 : 1]) {
   f2 all = both(0.f);
 #pragma unroll
   for (int j = 0; j < N2; ++j) {
-    x[j] = mul2(l[j], both(a.inv_cap));
     float da, db;
-    const f2 q = mul2(x[j], x[j]);
+    const f2 x = mul2(score(j), both(a.inv_cap)), q = mul2(x, x);
     all = add2(all, q);
     split(fma2(q, fma2(q, both(15.f), both(420.f)), both(945.f)), da, db);
-    const f2 t = mul2(mul2(x[j], fma2(q, add2(q, both(105.f)), both(945.f))), pair(fast_rcp(da), fast_rcp(db)));
+    const f2 t = mul2(mul2(x, fma2(q, add2(q, both(105.f)), both(945.f))), pair(fast_rcp(da), fast_rcp(db)));
     l[j] = mul2(t, both(a.scale));
     if (GRAD) d[j] = mul2(fma2(mul2(t, both(-1.f)), t, both(1.f)), both(a.scale * a.inv_cap));
   }
   if (!__any_sync(0xffffffffu, !(sum2(all) <= 1.f))) return;
 #pragma unroll
   for (int j = 0; j < N2; ++j) {
-    float v[2], lj[2], dj[2] = {0.f, 0.f};
-    split(x[j], v[0], v[1]);
+    float s[2], lj[2], dj[2] = {0.f, 0.f};
+    split(score(j), s[0], s[1]);
     split(l[j], lj[0], lj[1]);
     if (GRAD) split(d[j], dj[0], dj[1]);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const float e = fast_exp2(fabsf(v[h]) * (-2.f * kLog2e)), i = fast_rcp(1.f + e);
-      if (fabsf(v[h]) > 1.f) {
-        lj[h] = v[h] == -INFINITY ? -INFINITY : copysignf(fmaf(-2.f * e, i, 1.f), v[h]) * a.scale;
+      const float v = s[h] * a.inv_cap, e = fast_exp2(fabsf(v) * (-2.f * kLog2e)), i = fast_rcp(1.f + e);
+      if (fabsf(v) > 1.f) {
+        lj[h] = s[h] == -INFINITY ? -INFINITY : copysignf(fmaf(-2.f * e, i, 1.f), v) * a.scale;
         dj[h] = 4.f * e * i * i * (a.scale * a.inv_cap);
       }
     }
@@ -330,19 +329,22 @@ __global__ void __launch_bounds__(forward_threads(NC)) route_kernel(const __grid
     }
     const bool live = !K::empty(first);
     // logits of the chosen, then of all; the largest is the first chosen one's
+    const auto pick = [&](int i) {
+      return pair(K::value(mine[2 * i]), 2 * i + 1 < SL ? K::value(mine[2 * i + 1 < SL ? 2 * i + 1 : 0]) : 0.f);
+    };
+    const auto score = [&](int x) { return s[x / 4].get(x % 4); };
     f2 lm[(SL + 1) / 2], none[1];
 #pragma unroll
-    for (int i = 0; i < (SL + 1) / 2; ++i)
-      lm[i] = pair(K::value(mine[2 * i]), 2 * i + 1 < SL ? K::value(mine[2 * i + 1 < SL ? 2 * i + 1 : 0]) : 0.f);
-    if (a.rule == 1) cap_logits<(SL + 1) / 2, false>(a, lm, none);
+    for (int i = 0; i < (SL + 1) / 2; ++i) lm[i] = pick(i);
+    if (a.rule == 1) cap_logits<(SL + 1) / 2, false>(a, pick, lm, none);
     float la, lb;
     split(lm[0], la, lb);
     const float lead = __shfl_sync(0xffffffffu, la, lane - gl);
     const float top = live ? lead : 0.f;
     f2 ex[N / 2], sum = both(0.f);
 #pragma unroll
-    for (int x = 0; x < N / 2; ++x) ex[x] = s[x / 4].get(x % 4);
-    if (a.rule == 1) cap_logits<N / 2, false>(a, ex, none);
+    for (int x = 0; x < N / 2; ++x) ex[x] = score(x);
+    if (a.rule == 1) cap_logits<N / 2, false>(a, score, ex, none);
 #pragma unroll
     for (int x = 0; x < N / 2; ++x) {
       // (the difference first: exact for what matters, whatever the scores' size)
@@ -569,10 +571,11 @@ __global__ void __launch_bounds__(kRouteThreads, NC == 1 && G >= 16 ? 3 : 1) rou
       inner = fmaf(now.g[i], now.dg[i], inner);
       total += now.g[i];
     }
+    const auto score = [&](int x) { return now.s[x / 4].get(x % 4); };
     f2 p[N / 2], th[N / 2], dot2 = both(0.f);
 #pragma unroll
-    for (int x = 0; x < N / 2; ++x) { p[x] = now.s[x / 4].get(x % 4); th[x] = both(1.f); }
-    if (a.rule == 1) cap_logits<N / 2, true>(a, p, th);
+    for (int x = 0; x < N / 2; ++x) { p[x] = score(x); th[x] = both(1.f); }
+    if (a.rule == 1) cap_logits<N / 2, true>(a, score, p, th);
 #pragma unroll
     for (int x = 0; x < N / 2; ++x) {
       float la, lb;
@@ -653,9 +656,12 @@ int check_route(const tmoe_route_t *p) {
     return TMOE_ERR_SHAPE;
   if (p->n_experts > kRouteMaxExperts) return TMOE_ERR_UNSUPPORTED;
   if (p->router_mode != TMOE_ROUTER_TOPK_SOFTMAX && p->router_mode != TMOE_ROUTER_CAPPED_SOFTMAX) return TMOE_ERR_UNSUPPORTED;
-  if (p->router_mode == TMOE_ROUTER_CAPPED_SOFTMAX &&
-      (!(p->router_cap > 0.f) || !(p->router_temperature > 0.f) || std::isinf(p->router_cap) || std::isinf(p->router_temperature)))
-    return TMOE_ERR_SHAPE;
+  if (p->router_mode == TMOE_ROUTER_CAPPED_SOFTMAX) {
+    const float cap = p->router_cap, temperature = p->router_temperature;
+    if (!(cap > 0.f) || !(temperature > 0.f) || std::isinf(cap) || std::isinf(temperature)) return TMOE_ERR_SHAPE;
+    // what the kernels multiply by; an infinite one would make NaN of a score of 0, a subnormal one has lost its digits
+    if (!std::isnormal(1.f / cap) || !std::isnormal(cap / temperature) || !std::isnormal(1.f / temperature)) return TMOE_ERR_SHAPE;
+  }
   if (p->tokens == 0) return TMOE_OK;
   if (!p->scores) return TMOE_ERR_NULL;
   if (reinterpret_cast<uintptr_t>(p->scores) & (p->dtype == TMOE_F32 ? 3 : 1)) return TMOE_ERR_ALIGN;

@@ -70,7 +70,9 @@ def route(**kw):
     (dict(n_experts=1025), UNSUPPORTED), (dict(router_mode=2), UNSUPPORTED), (dict(dtype=5), DTYPE), (dict(scores=None), NULL),
     (dict(scores=P + 1), ALIGN), (dict(dtype=0, scores=P + 2), ALIGN), (dict(router_mode=1, router_cap=0.0), SHAPE),
     (dict(router_mode=1, router_cap=float("nan")), SHAPE), (dict(router_mode=1, router_temperature=float("inf")), SHAPE),
-    (dict(router_mode=1, router_temperature=-1.0), SHAPE),
+    (dict(router_mode=1, router_temperature=-1.0), SHAPE), (dict(router_mode=1, router_cap=1e-39), SHAPE),
+    (dict(router_mode=1, router_cap=3e38), SHAPE), (dict(router_mode=1, router_temperature=1e-39), SHAPE),
+    (dict(router_mode=1, router_cap=1e25, router_temperature=1e-20), SHAPE), (dict(router_mode=1, router_cap=1e-25, router_temperature=1e20), SHAPE),
 ])
 def test_route_refusals(kw, code):
     lib, p = _lib.load(), route(**kw)

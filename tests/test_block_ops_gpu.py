@@ -348,6 +348,19 @@ def test_route_lowest_finite_scores_are_scores():
         assert r.idx.tolist() == [[0, 1], [4, 0], [3, 2]] and bool(torch.isfinite(r.gates).all())
 
 
+def test_route_caps_far_from_one():
+    """Caps so small that finite scores overflow when divided by them (they stay on, at the end of the tanh), and so large that the cap
+    does nothing."""
+    s, mask, ups = route_inputs(20, 24, 4, F32, spread=1.0)
+    s[3, 5], s[3, 6], s[4, 7] = -3e38, 3e38, -3e38
+    s[5] = -3e38
+    s[6, 2] = -torch.inf
+    for cap, temp in ((0.25, 2.0), (1e-3, 0.5)):
+        check_route(s, None, ups, 4, 1, cap=cap, temp=temp)
+    t, _, ups = route_inputs(20, 24, 4, F32, spread=1.0)
+    check_route(t, None, ups, 4, 1, cap=1e6, temp=1.0)
+
+
 def test_route_ties_signed_zeros_and_nan():
     s = torch.zeros(4, 20)
     s[1, 3:] = -0.0
