@@ -6,7 +6,8 @@
 
 All three are differentiable.  They call the C-ABI library on the caller's current stream, allocate their results and scratch
 from torch's allocator on it (nothing is kept between calls, so captured graphs share no scratch) and run on CUDA tensors only.
-Results are bit-reproducible.  Gradients of gradients are not implemented.
+Results are bit-reproducible.  Gradients of gradients are not implemented.  Capture a backward pass on leaves that no eager autograd
+graph still holds, as everywhere in torch: the leaves' accumulators belong to the stream of the first graph that uses them.
 """
 from __future__ import annotations
 
@@ -362,7 +363,9 @@ class _RouteTokens(torch.autograd.Function):
         ctx.mark_non_differentiable(idx, counts)
         ctx.save_for_backward(scores, mask, idx, gates, counts, losses, stats)
         ctx.top_k, ctx.router = top_k, router
-        return idx, gates, counts, losses[0], losses[1]
+        # .data: results of their own, not views of a saved tensor, so that `loss += ...` may change them in place (the backward call reads
+        # the token count behind them only)
+        return idx, gates, counts, losses[0].data, losses[1].data
 
     @staticmethod
     @_first_order

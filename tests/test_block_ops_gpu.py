@@ -159,6 +159,28 @@ def test_norm_only_one_upstream_gradient_and_frozen_inputs():
     assert x["y"].grad is None
 
 
+def test_norm_one_tensor_in_several_places():
+    """y as its own residual and gate, one weight in three places: the gradient is the sum of the places'."""
+    for dtype in (BF, F32):
+        t, ups = norm_inputs(130, 768, dtype)
+        x, w = t["y"].cuda(), t["post"].cuda()
+        ups = [ups["d_out"].cuda(), ups["d_normed"].cuda()]
+
+        def run(y, residual, gate, scale, post, nxt):
+            got = residual_norm(y, residual=residual, gate=gate, layer_scale=scale, post_norm=(post, 1e-6), next_norm=(nxt, 1e-5))
+            return got, lambda leaves: torch.autograd.grad(got, leaves, ups)
+        y1, w1 = x.clone().requires_grad_(), w.clone().requires_grad_()
+        one, grad_one = run(y1, y1, y1, w1, w1, w1)
+        many = [a.clone().requires_grad_() for a in (x, x, x, w, w, w)]
+        apart, grad_apart = run(*many)
+        assert all(torch.equal(a, b) for a, b in zip(one, apart))
+        (gy, gw), g = grad_one([y1, w1]), grad_apart(many)
+        eps = torch.finfo(dtype).eps          # two additions of autograd's, each rounded by half a step of a partial sum
+        for got, parts in ((gy, g[:3]), (gw, g[3:])):
+            exact, size = sum(q.double() for q in parts), sum(q.double().abs() for q in parts)
+            assert bool(((got.double() - exact).abs() <= size * eps * (1 + eps) + 1e-30).all())
+
+
 def test_norm_plain_rmsnorm_with_a_gradient():
     """Only next_norm: out is y itself, normed is the layer's own rms_norm to one rounding, and it has a gradient."""
     t, ups = norm_inputs(9, 768, BF, residual=False, gate=False, scale=False, post=False)
@@ -412,6 +434,22 @@ def test_route_each_upstream_gradient_alone():
             r = route_tokens(x, 3, token_mask=mask.cuda(), router=(rule, 10.0, 0.5))
             (r.gates, r.balance_loss, r.z_loss)[i].backward(ups[i].cuda())
             near(f"d_scores from output {i}", x.grad, want["scores"])
+
+
+def test_route_losses_may_be_changed_in_place():
+    """The weighted sum of the losses, gathered in place as training code does."""
+    s, mask, ups = route_inputs(700, 64, 2, F32, padded=True)
+    want = ora.routing(s, 2, mask, (0, 10.0, 0.5), None, torch.tensor(0.5), torch.tensor(0.25))
+    x = s.cuda().requires_grad_()
+    r = route_tokens(x, 2, token_mask=mask.cuda())
+    before = [r.balance_loss.detach().clone(), r.z_loss.detach().clone()]
+    loss = r.balance_loss
+    loss *= 2.0
+    loss += r.z_loss
+    r.z_loss.zero_()
+    assert torch.equal(loss.detach(), 2.0 * before[0] + before[1])
+    loss.backward(torch.tensor(0.25).cuda())
+    near("d_scores", x.grad, want["scores"])
 
 
 def test_route_gradient_against_differences():
