@@ -213,9 +213,9 @@ int tmoe_rms_norm(int dtype, const void *x, const void *weight, float eps, int64
                   void *stream);
 
 /* ---- What stands around the layer in a block: its tail, its routing as data, its coefficients --------------------
- * Forward and backward.  Pointers need the alignment of their elements only (16-byte aligned rows of a multiple of 8 elements
- * take wider loads); last dimensions are contiguous, rows may lie any non-negative stride apart (0 repeats one row).  Outputs
- * are dense.  Workspaces of these functions are scratch of one call: never zeroed, nothing is kept in them. */
+ * Forward and backward.  Pointers need the alignment of their elements only (rows that start 16-byte aligned, fp32 rows
+ * of the tail 32-byte aligned, and hold a multiple of 8 elements take wider loads); last dimensions are contiguous, rows may lie
+ * any non-negative stride apart (0 repeats one row).  Outputs are dense.  Workspaces of these functions are scratch of one call: never zeroed, nothing is kept in them. */
 
 /* The tail of a block (pure_torch_mlx/model.py:25-27, 258-260, 340-341), with an optional norm behind the block:
  *   out    = residual + layer_scale * silu(gate) * (y * rstd(y) * post_w)
@@ -271,7 +271,8 @@ int64_t tmoe_route_workspace_bytes(const tmoe_route_t *p);   /* of the forward c
 int tmoe_route_tokens(const tmoe_route_t *p, int32_t *idx, float *gates, int32_t *counts, float *losses, float *stats, void *workspace,
                       int64_t workspace_bytes, void *stream);
 /* d_scores [tokens, n_experts] (dtype) from the forward call's results and the upstream gradients d_gates [tokens, top_k],
- * d_balance and d_z (one float each, on the device); each may be NULL (zero).  counts carry no gradient. */
+ * d_balance and d_z (one float each, on the device); each may be NULL (zero).  counts carry no gradient.  Of losses only the
+ * number of tokens is read. */
 int tmoe_route_tokens_backward(const tmoe_route_t *p, const int32_t *idx, const float *gates, const int32_t *counts,
                                const float *losses, const float *stats, const float *d_gates, const float *d_balance,
                                const float *d_z, void *d_scores, void *stream);
