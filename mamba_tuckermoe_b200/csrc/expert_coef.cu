@@ -20,6 +20,7 @@ namespace {
 constexpr int kCoefMaxExperts = 8192;    // a table of 4 columns: 128 KB
 constexpr int kCoefSmem = 192 * 1024;    // shared memory for the tables of one block
 constexpr int kDuThreads = 640;          // 20 warps of up to 96 registers
+constexpr int kDuClear = 512;            // threads that clear and fold the tables at least
 constexpr int kAhead = 4;                // rounds of slots whose operands are in flight
 
 struct CoefArgs {
@@ -142,8 +143,8 @@ __global__ void __launch_bounds__(256) coef_d_gates_kernel(const __grid_constant
 
 // A group of S * L lanes (a power of two up to 32) takes S slots of a token at once, 4 columns a lane, with a private table.  The experts of
 // a token usually differ, so the S slots touch different rows of it; where an expert is given twice the lanes take turns.  The operands of
-// kAhead rounds are in flight while the ones before are added.  blockIdx.y picks the columns; threads beyond the last group only keep
-// their warp whole.  Bound by the rounds' read-modify-write on few warps (the tables fill shared memory): 131072 tokens x 8 slots, 256
+// kAhead rounds are in flight while the ones before are added.  blockIdx.y picks the columns; threads beyond the last group only
+// clear and fold tables.  Bound by the rounds' read-modify-write on few warps (the tables fill shared memory): 131072 tokens x 8 slots, 256
 // experts, r1 = 8 take 26 us, with one column a lane they took 38; 32768 x 2, 64 experts, r1 = 4 take 6 us.
 template <int L>
 __global__ void __launch_bounds__(kDuThreads) coef_d_u_kernel(const __grid_constant__ CoefArgs a, int S, int groups, int wide) {
@@ -197,7 +198,8 @@ __global__ void __launch_bounds__(kDuThreads) coef_d_u_kernel(const __grid_const
     v.x = fmaf(w, x.x, v.x); v.y = fmaf(w, x.y, v.y); v.z = fmaf(w, x.z, v.z); v.w = fmaf(w, x.w, v.w);
     mine[row * L] = v;
   };
-  for (int r = 0; r < rounds; r += kAhead) {
+  const bool idle = (int)(threadIdx.x & ~31u) >= groups * lanes;   // a warp without a group only clears and folds
+  for (int r = idle ? rounds : 0; r < rounds; r += kAhead) {
 #pragma unroll
     for (int q = 0; q < kAhead; ++q) { e[q] = e_next[q]; g[q] = g_next[q]; d[q] = d_next[q]; }
     if (r + kAhead < rounds) fetch();
@@ -224,12 +226,23 @@ __global__ void __launch_bounds__(kDuThreads) coef_d_u_kernel(const __grid_const
   __syncthreads();
   // the kernel before this one in the stream (d_gates, whose output nothing here reads) may still run until here
   ptx::griddep_wait();
-  const float *flat = reinterpret_cast<const float *>(tab);
-  for (int i = threadIdx.x; i < width * 4; i += blockDim.x) {
-    float v = 0.f;
-    for (int q = 0; q < groups; ++q) v += flat[q * width * 4 + i];
-    const int x = i / (L * 4), q = blockIdx.y * L * 4 + i - x * L * 4;
-    if (q < a.r1) a.partial[((int64_t)blockIdx.x * a.E + x) * a.r1 + q] = v;
+  for (int i = threadIdx.x; i < width; i += blockDim.x) {
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int q = 0; q < groups; ++q) {
+      const float4 w = tab[q * width + i];
+      v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+    }
+    const int x = i / L, q = (blockIdx.y * L + i - x * L) * 4;
+    float *to = a.partial + ((int64_t)blockIdx.x * a.E + x) * a.r1 + q;
+    if (a.r1 % 4 == 0) {
+      if (q < a.r1) *reinterpret_cast<float4 *>(to) = v;
+    } else {
+      const float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int y = 0; y < 4; ++y)
+        if (q + y < a.r1) to[y] = f[y];
+    }
   }
 }
 
@@ -291,7 +304,7 @@ int launch_d_u(const CoefArgs &a, const DuShape &s, bool overlap, cudaStream_t s
     if (cudaFuncSetAttribute(coef_d_u_kernel<L>, cudaFuncAttributeMaxDynamicSharedMemorySize, kCoefSmem) != cudaSuccess) return TMOE_ERR_CUDA;
     opted.fetch_or(bit, std::memory_order_relaxed);
   }
-  const int threads = (s.groups * s.S * s.L + 31) / 32 * 32, wide = a.r1 % 4 == 0 && !(reinterpret_cast<uintptr_t>(a.d_c) & 15);
+  const int need = (s.groups * s.S * s.L + 31) / 32 * 32, threads = need > kDuClear ? need : kDuClear, wide = a.r1 % 4 == 0 && !(reinterpret_cast<uintptr_t>(a.d_c) & 15);
   const size_t smem = (size_t)s.groups * a.E * s.L * 16;
   const dim3 grid((unsigned)s.blocks, (unsigned)s.parts), block((unsigned)threads);
   count_launch();
