@@ -146,24 +146,27 @@ __global__ void __launch_bounds__(256) coef_d_gates_kernel(const __grid_constant
 // kAhead rounds are in flight while the ones before are added.  blockIdx.y picks the columns; threads beyond the last group only
 // clear and fold tables.  Bound by the rounds' read-modify-write on few warps (the tables fill shared memory): 131072 tokens x 8 slots, 256
 // experts, r1 = 8 take 26 us, with one column a lane they took 38; 32768 x 2, 64 experts, r1 = 4 take 6 us.
-template <int L>
-__global__ void __launch_bounds__(kDuThreads) coef_d_u_kernel(const __grid_constant__ CoefArgs a, int S, int groups, int wide) {
+template <int L, int S>
+__global__ void __launch_bounds__(kDuThreads) coef_d_u_kernel(const __grid_constant__ CoefArgs a, int groups, int wide) {
+  constexpr int lanes = S * L;
   extern __shared__ __align__(16) float4 tab[];   // [groups][E * L]
-  const int lanes = S * L, grp = threadIdx.x / lanes, in = threadIdx.x - grp * lanes, lane = threadIdx.x & 31;
+  const int grp = threadIdx.x / lanes, in = threadIdx.x - grp * lanes, lane = threadIdx.x & 31;
   const int s = in / L, col = in - s * L, c = (blockIdx.y * L + col) * 4, width = a.E * L;
   ptx::griddep_launch_dependents();
   for (int i = threadIdx.x; i < groups * width; i += blockDim.x) tab[i] = make_float4(0.f, 0.f, 0.f, 0.f);
   // the lanes of this group that hold the same columns of the slots before this one
+  const int lane0 = (lane & ~(lanes - 1)) + col;
   uint32_t before = 0;
-  for (int q = 0; q < s; ++q) before |= 1u << ((lane & ~(lanes - 1)) + q * L + col);
+#pragma unroll
+  for (int q = 0; q < S; ++q) before |= q < s ? 1u << (lane0 + q * L) : 0u;
   const int64_t lo = a.T * blockIdx.x / gridDim.x, hi = a.T * (blockIdx.x + 1) / gridDim.x;
   // every lane of the block walks the same number of rounds: the turns need whole warps (rounds beyond the last are empty)
   const int rounds = (int)((hi - lo + groups - 1) / groups) * ((a.k + S - 1) / S);
   int left = grp < groups && c < a.r1 ? (int)((hi - lo - grp + groups - 1) / groups) : 0;   // tokens of this group
-  int j = s;
+  int base = 0;                                             // slots of the current token that are done
   const int64_t t0 = lo + (grp < groups ? grp : 0);
-  const int32_t *idx = a.idx + t0 * a.k;
-  const float *gates = a.gates + t0 * a.k, *d_c = a.d_c + t0 * a.r1 + c;
+  const int32_t *idx = a.idx + t0 * a.k + s;
+  const float *gates = a.gates + t0 * a.k + s, *d_c = a.d_c + t0 * a.r1 + c;
   const int64_t k_step = (int64_t)groups * a.k, d_step = (int64_t)groups * a.r1;
   int e_next[kAhead], e[kAhead];
   float g_next[kAhead], g[kAhead];
@@ -174,9 +177,9 @@ __global__ void __launch_bounds__(kDuThreads) coef_d_u_kernel(const __grid_const
       e_next[q] = -1;
       g_next[q] = 0.f;
       d_next[q] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (left > 0 && j < a.k) {
-        e_next[q] = __ldg(idx + j);
-        g_next[q] = __ldg(gates + j);
+      if (left > 0 && base + s < a.k) {
+        e_next[q] = __ldg(idx + base);
+        g_next[q] = __ldg(gates + base);
         if (wide) {
           d_next[q] = __ldg(reinterpret_cast<const float4 *>(d_c));
         } else {
@@ -186,8 +189,8 @@ __global__ void __launch_bounds__(kDuThreads) coef_d_u_kernel(const __grid_const
           if (c + 3 < a.r1) d_next[q].w = __ldg(d_c + 3);
         }
       }
-      j += S;
-      if (j - s >= a.k) { j = s; --left; idx += k_step; gates += k_step; d_c += d_step; }
+      base += S;
+      if (base >= a.k) { base = 0; --left; idx += k_step; gates += k_step; d_c += d_step; }
     }
   };
   fetch();
@@ -207,8 +210,9 @@ __global__ void __launch_bounds__(kDuThreads) coef_d_u_kernel(const __grid_const
     for (int q = 0; q < kAhead; ++q) {
       const bool have = (unsigned)e[q] < (unsigned)a.E;
       bool twice = false;
-      for (int o = L; o < lanes; o += L) {
-        const int other = __shfl_xor_sync(0xffffffffu, e[q], o);   // by every lane, whatever it has found
+#pragma unroll
+      for (int o = 1; o <= S / 2; ++o) {   // of every two slots one sees the other; by every lane, whatever it has found
+        const int other = __shfl_sync(0xffffffffu, e[q], lane0 + (s + o) % S * L);
         twice |= other == e[q];
       }
       if (!__any_sync(0xffffffffu, have && twice)) {
@@ -294,24 +298,35 @@ DuShape du_shape(int64_t T, int E, int k, int r1, int sms) {
   return s;
 }
 
-template <int L>
-int launch_d_u(const CoefArgs &a, const DuShape &s, bool overlap, cudaStream_t st) {
+template <int L, int S>
+int launch_d_u_as(const CoefArgs &a, const DuShape &s, bool overlap, cudaStream_t st) {
   static std::atomic<uint64_t> opted{0};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return TMOE_ERR_CUDA;
   const uint64_t bit = 1ull << (dev & 63);
   if (!(opted.load(std::memory_order_relaxed) & bit)) {
-    if (cudaFuncSetAttribute(coef_d_u_kernel<L>, cudaFuncAttributeMaxDynamicSharedMemorySize, kCoefSmem) != cudaSuccess) return TMOE_ERR_CUDA;
+    if (cudaFuncSetAttribute(coef_d_u_kernel<L, S>, cudaFuncAttributeMaxDynamicSharedMemorySize, kCoefSmem) != cudaSuccess) return TMOE_ERR_CUDA;
     opted.fetch_or(bit, std::memory_order_relaxed);
   }
-  const int need = (s.groups * s.S * s.L + 31) / 32 * 32, threads = need > kDuClear ? need : kDuClear, wide = a.r1 % 4 == 0 && !(reinterpret_cast<uintptr_t>(a.d_c) & 15);
-  const size_t smem = (size_t)s.groups * a.E * s.L * 16;
+  const int need = (s.groups * S * L + 31) / 32 * 32, threads = need > kDuClear ? need : kDuClear, wide = a.r1 % 4 == 0 && !(reinterpret_cast<uintptr_t>(a.d_c) & 15);
+  const size_t smem = (size_t)s.groups * a.E * L * 16;
   const dim3 grid((unsigned)s.blocks, (unsigned)s.parts), block((unsigned)threads);
   count_launch();
   // after d_gates of the same call it may begin while that runs: both only read what was there before
-  if (overlap) return cuda_ok(launch_pdl(coef_d_u_kernel<L>, grid, block, smem, st, a, s.S, s.groups, wide));
-  coef_d_u_kernel<L><<<grid, block, smem, st>>>(a, s.S, s.groups, wide);
+  if (overlap) return cuda_ok(launch_pdl(coef_d_u_kernel<L, S>, grid, block, smem, st, a, s.groups, wide));
+  coef_d_u_kernel<L, S><<<grid, block, smem, st>>>(a, s.groups, wide);
   return launch_status();
+}
+template <int L>
+int launch_d_u(const CoefArgs &a, const DuShape &s, bool overlap, cudaStream_t st) {
+  switch (s.S) {   // S * L is at most 32
+    case 1: return launch_d_u_as<L, 1>(a, s, overlap, st);
+    case 2: return launch_d_u_as<L, 2>(a, s, overlap, st);
+    case 4: if constexpr (L <= 8) return launch_d_u_as<L, 4>(a, s, overlap, st); break;
+    case 8: if constexpr (L <= 4) return launch_d_u_as<L, 8>(a, s, overlap, st); break;
+    case 16: if constexpr (L <= 2) return launch_d_u_as<L, 16>(a, s, overlap, st); break;
+  }
+  return TMOE_ERR_UNSUPPORTED;
 }
 
 // wide: rows of U_expert, c and d_c are whole 4-column pieces
