@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(256) coef_d_gates_kernel(const __grid_constant
 // a token usually differ, so the S slots touch different rows of it; where an expert is given twice the lanes take turns.  The operands of
 // kAhead rounds are in flight while the ones before are added.  blockIdx.y picks the columns; threads beyond the last group only
 // clear and fold tables.  Bound by the rounds' read-modify-write on few warps (the tables fill shared memory): 131072 tokens x 8 slots, 256
-// experts, r1 = 8 take 26 us, with one column a lane they took 38; 32768 x 2, 64 experts, r1 = 4 take 6 us.
+// experts, r1 = 8 take 17 us, with the lane layout as arguments of the kernel they took 25; 32768 x 2, 64 experts, r1 = 4 take 6 us.
 template <int L, int S>
 __global__ void __launch_bounds__(kDuThreads) coef_d_u_kernel(const __grid_constant__ CoefArgs a, int groups, int wide) {
   constexpr int lanes = S * L;
