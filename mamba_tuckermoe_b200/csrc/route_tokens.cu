@@ -334,17 +334,23 @@ __global__ void __launch_bounds__(forward_threads(NC)) route_kernel(const __grid
     };
     const auto score = [&](int x) { return s[x / 4].get(x % 4); };
     f2 lm[(SL + 1) / 2], none[1];
+    if (a.rule == 1) {
+      cap_logits<(SL + 1) / 2, false>(a, pick, lm, none);
+    } else {
 #pragma unroll
-    for (int i = 0; i < (SL + 1) / 2; ++i) lm[i] = pick(i);
-    if (a.rule == 1) cap_logits<(SL + 1) / 2, false>(a, pick, lm, none);
+      for (int i = 0; i < (SL + 1) / 2; ++i) lm[i] = pick(i);
+    }
     float la, lb;
     split(lm[0], la, lb);
     const float lead = __shfl_sync(0xffffffffu, la, lane - gl);
     const float top = live ? lead : 0.f;
     f2 ex[N / 2], sum = both(0.f);
+    if (a.rule == 1) {
+      cap_logits<N / 2, false>(a, score, ex, none);
+    } else {
 #pragma unroll
-    for (int x = 0; x < N / 2; ++x) ex[x] = score(x);
-    if (a.rule == 1) cap_logits<N / 2, false>(a, score, ex, none);
+      for (int x = 0; x < N / 2; ++x) ex[x] = score(x);
+    }
 #pragma unroll
     for (int x = 0; x < N / 2; ++x) {
       // (the difference first: exact for what matters, whatever the scores' size)
@@ -573,9 +579,12 @@ __global__ void __launch_bounds__(kRouteThreads, NC == 1 && G >= 16 ? 3 : 1) rou
     }
     const auto score = [&](int x) { return now.s[x / 4].get(x % 4); };
     f2 p[N / 2], th[N / 2], dot2 = both(0.f);
+    if (a.rule == 1) {
+      cap_logits<N / 2, true>(a, score, p, th);
+    } else {
 #pragma unroll
-    for (int x = 0; x < N / 2; ++x) { p[x] = score(x); th[x] = both(1.f); }
-    if (a.rule == 1) cap_logits<N / 2, true>(a, score, p, th);
+      for (int x = 0; x < N / 2; ++x) { p[x] = score(x); th[x] = both(1.f); }
+    }
 #pragma unroll
     for (int x = 0; x < N / 2; ++x) {
       float la, lb;
