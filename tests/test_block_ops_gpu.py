@@ -535,6 +535,24 @@ def test_coef_sizes(T, E, k, r1):
     check_coef(*coef_inputs(T, E, k, r1, F32, hot=T == 1000))
 
 
+@pytest.mark.parametrize("k", [1, 2, 3, 4, 8, 9, 16])
+@pytest.mark.parametrize("r1", [4, 8, 12, 16, 32, 64])
+def test_coef_lane_layouts(k, r1):
+    """Every split of a warp into slots and columns, with experts repeated within a token, and enough tokens for several rounds."""
+    check_coef(*coef_inputs(203, 9, k, r1, F32))
+
+
+def test_coef_upstream_gradient_off_16_bytes():
+    idx, gates, u, d_c = coef_inputs(77, 40, 2, 8, F32)
+    want = ora.coefficients(idx, gates, u, d_c)
+    flat = torch.empty(d_c.numel() + 1, device="cuda")
+    flat[1:] = d_c.cuda().flatten()
+    g, w = gates.cuda().requires_grad_(), u.cuda().requires_grad_()
+    d_g, d_u = torch.autograd.grad(expert_coefficients(idx.cuda(), g, w), [g, w], flat[1:].view(77, 8))
+    near("d_gates", d_g, want["gates"])
+    near("d_U", d_u, want["u"])
+
+
 def test_coef_many_experts():
     check_coef(*coef_inputs(50, 8192, 2, 4, F32))
     check_coef(*coef_inputs(50, 1024, 2, 64, BF))
