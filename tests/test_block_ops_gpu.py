@@ -104,6 +104,36 @@ def test_norm_every_combination_of_operands(flags):
     check_norm(6, 99, F32, **kw)
 
 
+@pytest.mark.parametrize("rows,d", [(1, 8), (2, 8), (7, 24), (300, 8), (40000, 128), (2100, 2304), (900, 8192)])
+@pytest.mark.parametrize("dtype,res", [(BF, BF), (BF, F32), (F32, F32)])
+def test_tail_without_norms(rows, d, dtype, res):
+    """One piece a row to 1024, less than a grid of them and several; the last row against rows of a wider tensor too."""
+    for kw in (dict(scale=False, gate=False), dict(), dict(scale=False)):
+        t, ups = norm_inputs(rows, d, dtype, post=False, nxt=False, res_dtype=res, **kw)
+        want = ora.norm_tail(t["y"], t["residual"], t["gate"], t["layer_scale"], None, None, ups["d_out"], None)
+        for gap in (0, 8, 3):      # whole pieces, whole pieces apart, and rows that start anywhere (the row walk)
+            _, out, normed = run_norm(t, gap=gap, grad=False)
+            assert normed is None and out.dtype == res
+            near("out", out, want["out"])
+
+
+def test_tail_without_norms_beyond_32_bit_offsets_and_over_its_residual():
+    import ctypes as C
+    from mamba_tuckermoe_b200 import _lib
+    rows, d = 2 ** 31 // 8192 + 200, 8192
+    y = torch.empty(rows, d, dtype=BF, device="cuda")
+    y[-200:] = torch.randn(200, d, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+    w = torch.rand(d, device="cuda").to(BF)
+    out, _ = residual_norm(y, layer_scale=w)
+    assert torch.equal(out[-200:], residual_norm(y[-200:].clone(), layer_scale=w)[0])
+    del out
+    y = y[-200:].clone()
+    res = torch.randn(200, d, device="cuda").to(BF)
+    want, _ = residual_norm(y, residual=res, layer_scale=w)
+    p = _lib.ResidualNorm(200, d, _lib.TMOE_BF16, _lib.TMOE_BF16, 0.0, 0.0, 0, d, d, 0, y.data_ptr(), res.data_ptr(), None, w.data_ptr(), None, None)
+    assert _lib.load().tmoe_residual_norm(C.byref(p), res.data_ptr(), None, None, _lib.current_stream_ptr()) == 0 and torch.equal(res, want)
+
+
 @pytest.mark.parametrize("d", [96, 768, 1003, 2304, 6144])
 def test_norm_residual_stream_in_fp32(d):
     check_norm(21, d, BF, res_dtype=F32)
