@@ -33,10 +33,13 @@ namespace {
 
 constexpr int kMaxWidth = 8192;      // widest row: 512 threads x 16 elements
 // Warps that an SM is meant to hold, by the registers a thread needs.  Forward 32 (64 registers) in blocks of 8 or of one row each;
-// backward one block of 20 (96 registers), or 16 (128) in fp32; 16 where a thread has 16 elements.
-constexpr int resident_warps(int nv, bool back, bool f32) { return nv == 2 ? 16 : back ? (f32 ? 16 : 20) : 32; }
+// backward one block of 20 (96 registers), or 16 (128) in fp32; 16 where a thread has 16 elements, 18 (96 registers) in the fp32 forward without
+// a gate, so that two blocks of 9 fit (4608 columns: 51 us against 75).
+constexpr int resident_warps(int nv, bool back, bool f32, bool gate) {
+  return nv == 2 ? (f32 && !back && !gate ? 18 : 16) : back ? (f32 ? 16 : 20) : 32;
+}
 // Warps of the largest block
-constexpr int block_warps(int nv, bool back, bool f32) { return back ? resident_warps(nv, back, f32) : 16; }
+constexpr int block_warps(int nv, bool back, bool f32) { return back ? resident_warps(nv, back, f32, true) : 16; }
 constexpr int kMaxTeams = 10;           // teams of several warps in a block (a named barrier each)
 constexpr int kRingBytes = 208 * 1024;
 
@@ -210,10 +213,13 @@ template <typename TY, typename TR, int VEC, int NV, bool GATE, bool BACK> struc
   using PR = Piece<TR, VEC>;
   static constexpr int kPlanes = NV * ((1 + (GATE ? 1 : 0) + (BACK ? 1 : 0)) * PY::kPlanes + (BACK ? 2 : 1) * PR::kPlanes);
   // as many rows ahead as fit for the warps that an SM is meant to run; below 2 stages rows are loaded when their turn comes
-  // (backward, the parameters' columns of a thread lie behind the ring, in fp32)
+  // (backward, the parameters' columns of a thread lie behind the ring, in fp32).  The fp32 forward loads without a ring: its 32-byte pieces
+  // keep as much in flight from registers (18.9 M elements with a gate, 2304 columns: 60.5 us against 70.9 with a ring, 768: 59.3 / 70.8, 8192:
+  // 70.1 / 83.1, without a gate 1520: 49.4 / 58.1; only the gated blocks of 9 to 15 warps lose, 4608: 84.2 / 79.5); bf16 needs it (37.7 M elements of
+  // 2304 columns: 49.4 us against 73.8 without).
   static constexpr int kParamPlanes = BACK && VEC == 8 ? 4 * NV : 0;
-  static constexpr int kFit = kPlanes ? (kRingBytes / (resident_warps(NV, BACK, sizeof(TY) == 4) * 512) - kParamPlanes) / kPlanes : 0;
-  static constexpr int kStages = kFit >= 3 ? 3 : kFit == 2 ? 2 : 1;
+  static constexpr int kFit = kPlanes ? (kRingBytes / (resident_warps(NV, BACK, sizeof(TY) == 4, GATE) * 512) - kParamPlanes) / kPlanes : 0;
+  static constexpr int kStages = sizeof(TY) == 4 && !BACK ? 1 : kFit >= 3 ? 3 : kFit == 2 ? 2 : 1;
   static constexpr bool kRing = kStages > 1;
   PY y[NV], g[GATE ? NV : 1], dn[BACK ? NV : 1];
   PR r[NV], dout[BACK ? NV : 1];
@@ -355,7 +361,7 @@ template <typename TY, int VEC, int NV> struct Params {
 // A team walks over rows blockIdx * teams + team, + gridDim * teams, ...  Bound by memory: 32768 x 768 bf16 with every operand in 43 us
 // = 5.8 TB/s of 252 MB, 16384 x 2304 without a gate in 50 us = 6.1 TB/s.
 template <typename TY, typename TR, int VEC, int NV, bool GATE>
-__global__ void __launch_bounds__(512, VEC == 8 && NV == 1 ? 2 : 1) residual_norm_kernel(const __grid_constant__ NormArgs a) {
+__global__ void __launch_bounds__(VEC == 8 && NV == 2 && sizeof(TY) == 4 && !GATE ? 576 : 512, VEC == 8 && NV == 1 ? 2 : 1) residual_norm_kernel(const __grid_constant__ NormArgs a) {
   using In = RowIn<TY, TR, VEC, NV, GATE, false>;
   __shared__ __align__(16) TeamRed<1> red;
   ptx::griddep_launch_dependents();
@@ -605,7 +611,7 @@ NormShape norm_shape(const tmoe_residual_norm_t &p, bool back, int sms) {
   const bool two = back ? pieces > 128 && !f32 && p.residual_dtype == TMOE_BF16 && !p.gate : pieces > 64;
   s.nv = pieces > 32 * block_warps(1, back, f32) || (two && rows > sms) ? 2 : 1;
   s.tw = (pieces + 32 * s.nv - 1) / (32 * s.nv);
-  const int resident = resident_warps(s.nv, back, f32), full = back ? resident : 8;
+  const int resident = resident_warps(s.nv, back, f32, p.gate != nullptr), full = back ? resident : 8;
   s.teams = s.tw >= full ? 1 : full / s.tw;
   if (s.tw > 1 && s.teams > kMaxTeams) s.teams = kMaxTeams;
   const int64_t each = (rows + sms - 1) / sms;
