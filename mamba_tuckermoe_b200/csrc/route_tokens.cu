@@ -254,7 +254,7 @@ __device__ __forceinline__ void write_losses(const RouteArgs &a, float dot, floa
 // A lane sorts its keys once and leaves them in shared memory, so that a round of the selection is one maximum over the lanes' heads and one
 // load by the winner (shifting the list in registers instead kept the integer pipe busy for two thirds of the kernel).
 // Blocks write one row of partial sums each; a block that is alone finishes the losses itself.  Bound by instruction issue (78 % of the
-// slots): 131072 tokens x 256 bf16 scores, k = 8, rule 1 take 467 instructions a token, 67 us (and 9 us of losses), where reading the
+// slots): 131072 tokens x 256 bf16 scores, k = 8, rule 1 take 460 instructions a token, 67 us (and 9 us of losses), where reading the
 // scores alone is 10 us; 32768 x 64, k = 2 take 11 us in all.
 template <typename TS, int G, int NC, int DEPTH, bool WIDE>
 __global__ void __launch_bounds__(forward_threads(NC)) route_kernel(const __grid_constant__ RouteArgs a) {
@@ -509,7 +509,7 @@ __global__ void __launch_bounds__(kLossThreads) route_losses_kernel(const __grid
 
 // p comes from the kept largest logit and sum, so a token needs one pass over its row.  The gates' parts of the gradient go through a row of shared memory
 // per token: the lanes that hold slots put them at their columns, and every lane picks up its own eight.  131072 x 256 bf16, rule 1: 62 us for
-// 147 MB, 345 instructions a token in 66 % of the issue slots.
+// 147 MB, 327 instructions a token in about 65 % of the issue slots.
 template <typename TS, int G, int NC, bool WIDE>
 __global__ void __launch_bounds__(kRouteThreads, NC == 1 && G >= 16 ? 3 : 1) route_backward_kernel(const __grid_constant__ RouteArgs a) {
   constexpr int N = NC * 8, SL = Slots<G>::N, PER = 32 / G;
